@@ -350,6 +350,64 @@ int unetk_clip_rmsprop_step(float* param, float* grad, float* square_avg, float*
                             void* workspace, int64_t workspace_bytes, double* total_norm_out, float max_norm, float lr,
                             float alpha, float eps, float weight_decay, float momentum, void* stream);
 
+/* ---- optimizer step over many tensors -------------------------------------------------------------------------
+ * AdamW (decoupled weight decay) with a global-norm clip in front, over any number of parameter tensors at once; the
+ * tensors need not lie in one buffer, may have any number of elements (0 included) and any element-aligned address.
+ * No reference counterpart: the reference trains with RMSprop (train.py:77-78); the clip is its train.py:115.
+ *
+ * `tensors` is a HOST array that is read during the call (its contents travel as kernel arguments, so a captured graph
+ * replays the pointers it was captured with).  A call serves tensors of one element type (`dtype`: parameter and
+ * gradient); elements are taken in memory order, so all arrays of a tensor share one dense layout.
+ *   coef = min(1, max_norm / (norm + 1e-6)), norm = sqrt(sum of the partials) / grad_scale   (no partials: coef = 1)
+ *   g = coef * grad / grad_scale;  step += 1;  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2
+ *   param = param (1 - lr wd) - lr / (1 - b1^step) * m / (sqrt(v) / sqrt(1 - b2^step) + eps)
+ * The gradient is left as it is.  Moments and all arithmetic are fp32 (the partial sums and bias corrections fp64);
+ * a parameter of 16 bits is rounded once, to nearest.
+ *
+ * Moments in 8 bits (unetk_adamw8_update): a block is 256 consecutive elements of a tensor, the last one shorter.
+ * exp_avg holds m and exp_avg_sq holds the ROOT r = sqrt(v) as fp8 e4m3 codes of value / 2^k; `scales` holds 127 + k in a byte,
+ * [blocks][2]: m's and r's.  k is the smallest integer >= -127 with |value| <= 448 * 2^k for the block's finite values.
+ * Codes are rounded stochastically, |code| = floor(|x| / ulp + (u + 1/2) / 65536) * ulp with ulp the e4m3 spacing at
+ * x = value / 2^k: rounding to nearest would freeze r, which moves by (1 - b2) / 2 of itself a step where codes lie 6 to
+ * 12 % apart.  u is 16 bits of a hash: key = mix(seed + 0x9E3779B9 * step), h = mix(key ^ low ^ high 32 bits of the
+ * element's index), h's low half for m and its high half for r; mix(h) is two rounds of xor-shift and multiplication.  A
+ * root above zero never gets code zero (the next update would divide by eps alone).  A value that is not finite is stored
+ * as NaN and leaves its block's others alone.  The step itself uses m and v before they are rounded.  All bytes zero is a
+ * state of zeros.
+ *
+ * A step is two calls per set of tensors, and every unetk_adamw_prepare of a step comes before its first update:
+ * unetk_adamw_prepare: adds 1 to every `step`, writes each tensor's bias corrections to `coefs` (16 bytes a tensor) and, if
+ *   `partials` is not NULL, sums of squares of the gradients to `partials`.  Returns how many of them it wrote (at most
+ *   unetk_grad_partials(n_tensors)) or a negative error.  lr_dev (may be NULL): lr is read from there.
+ * unetk_adamw_update / unetk_adamw8_update: the update; `partials`, `n_partials`: those of ALL sets that the norm covers
+ *   (NULL and 0 without a clip).  norm_out (may be NULL) receives the norm.
+ * grad_scale, found_inf (device, may be NULL): torch.amp.GradScaler's; found_inf != 0 skips the step, its count included.
+ *
+ * unetk_grad_sumsq + unetk_grad_clip: torch.nn.utils.clip_grad_norm_ (reference train.py:115) by themselves, gradients
+ * scaled in place (not written where coef is 1); they read `grad` and `numel` of the records only. */
+typedef struct {
+  void* param;
+  void* grad;
+  void* exp_avg;    /* fp32, or e4m3 codes */
+  void* exp_avg_sq; /* fp32, or e4m3 codes of its root */
+  void* scales;     /* 8-bit moments: [ceil(numel / 256)][2] bytes */
+  float* step;
+  int64_t numel;
+} unetk_adamw_tensor;
+int64_t unetk_grad_partials(int n_tensors);
+int64_t unetk_grad_sumsq(const unetk_adamw_tensor* tensors, int n_tensors, int dtype, double* partials, void* stream);
+int unetk_grad_clip(const unetk_adamw_tensor* tensors, int n_tensors, int dtype, const double* partials,
+                    int64_t n_partials, double max_norm, float* norm_out, void* stream);
+int64_t unetk_adamw_prepare(const unetk_adamw_tensor* tensors, int n_tensors, int dtype, double lr, const float* lr_dev,
+                            double beta1, double beta2, double weight_decay, int64_t seed, const float* found_inf,
+                            float* coefs, double* partials, void* stream);
+int unetk_adamw_update(const unetk_adamw_tensor* tensors, int n_tensors, int dtype, double beta1, double beta2,
+                       double eps, const float* grad_scale, const float* found_inf, const float* coefs,
+                       const double* partials, int64_t n_partials, double max_norm, float* norm_out, void* stream);
+int unetk_adamw8_update(const unetk_adamw_tensor* tensors, int n_tensors, int dtype, double beta1, double beta2,
+                        double eps, const float* grad_scale, const float* found_inf, const float* coefs,
+                        const double* partials, int64_t n_partials, double max_norm, float* norm_out, void* stream);
+
 /* ---- input formatting: BasicDataset.preprocess, utils/data_loading.py:65-91 ----------
  * The reference resizes on the CPU with Pillow (`pil_img.resize`, :69: BICUBIC for images, NEAREST for masks) and
  * converts (:72-91).  These entry points do the same on decoded uint8 pixels already in HBM, BIT-EXACTLY

@@ -26,7 +26,7 @@ lib = ctypes.CDLL(LIB_PATH)
 
 HEADER_PATH = os.path.join(os.path.dirname(os.path.dirname(_HERE)), 'include', 'unetk.h')
 
-_CTYPE = {'int': ctypes.c_int, 'int64_t': ctypes.c_int64, 'float': ctypes.c_float}
+_CTYPE = {'int': ctypes.c_int, 'int64_t': ctypes.c_int64, 'float': ctypes.c_float, 'double': ctypes.c_double}
 
 
 def parse_header(path=HEADER_PATH):

@@ -7,11 +7,17 @@ nn.Parameter objects, same state_dict) at views of ONE flat fp32 buffer laid out
 buffer of unetk.ddp.FlatGrads, the optimizer state is two more flat buffers, and a step is two kernels
 (include/unetk.h: unetk_clip_rmsprop_step).  Subclasses torch.optim.Optimizer so LR schedulers
 (train.py:79 ReduceLROnPlateau) keep working through param_groups[0]['lr'].
+
+`AdamW` and `clip_grad_norm_` are the same step for other users' needs: any list of parameter tensors wherever they lie
+(or the flat buffers above), decoupled weight decay, moments in 32 or in 8 bits, the clip in front of the step or by itself.
 """
+import contextlib
+import ctypes
+
 import torch
 
 from . import _native as nat
-from ._native import check, fn, stream_ptr
+from ._native import check, dtype_code, fn, stream_ptr
 
 
 class ClipRMSprop(torch.optim.Optimizer):
@@ -132,3 +138,365 @@ class ClipRMSprop(torch.optim.Optimizer):
         self._steps += 1
         self.fg.consume()
         return None
+
+
+# ---------------------------------------------------------------------------------------- many tensors at once
+_WORDS = 7                      # unetk_adamw_tensor: param, grad, exp_avg, exp_avg_sq, scales, step, numel
+BLOCK = 256                     # elements that share one scale per moment (unetk_adamw8_update)
+_CODE, _SCALE = torch.float8_e4m3fn, torch.float8_e8m0fnu
+
+
+def _on_device(device):
+    """Launches go to the tensors' device whatever the current one is, on that device's current stream."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _is_dense(t):
+    """Whether the elements fill one piece of memory, in any order of the dimensions."""
+    if t.is_contiguous():
+        return True
+    expect = 1
+    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != expect:
+            return False
+        expect *= size
+    return True
+
+
+def _require(t, what, owner='AdamW'):
+    if t.layout != torch.strided:
+        raise RuntimeError(f'{owner}: {what} must be strided tensors, got {t.layout}')
+    if not t.is_cuda:
+        raise RuntimeError(f'{owner} runs on the MI355X kernels: {what} must be on a cuda device (no CPU fallback)')
+    dtype_code(t.dtype)
+    if not _is_dense(t):
+        raise RuntimeError(f'{owner}: {what} must be dense (no gaps, no overlaps), got strides {t.stride()} for shape '
+                           f'{tuple(t.shape)}')
+
+
+def _memory_order(t):
+    """The elements of a dense tensor as they lie in memory, as one dimension."""
+    return t.view(-1) if t.is_contiguous() else t.as_strided((t.numel(),), (1,))
+
+
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False, foreach=None):
+    """torch.nn.utils.clip_grad_norm_ (reference train.py:115) over any list of tensors in two passes: the 2-norm of all
+    gradients together, then every gradient times min(1, max_norm / (norm + 1e-6)) in place.  Gradients may be fp32, bf16 and
+    fp16 mixed; the sum of squares is taken in fp64.  Nothing is written where the norm is within the limit.  Returns the norm
+    as an fp32 scalar on the device; reads nothing back unless `error_if_nonfinite`.  `foreach` is accepted and ignored."""
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    if float(norm_type) != 2.0:
+        raise ValueError('clip_grad_norm_: only the 2-norm is implemented')
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise ValueError(f'clip_grad_norm_: max_norm must not be negative, got {max_norm}')
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if not grads:
+        return torch.tensor(0.0)
+    device = grads[0].device
+    by_type = {}
+    for g in grads:
+        _require(g, 'gradients', 'clip_grad_norm_')
+        if g.device != device:
+            raise RuntimeError('clip_grad_norm_: gradients must be on one device')
+        by_type.setdefault(g.dtype, []).append(g)
+    if len({id(g) for g in grads}) != len(grads):
+        raise ValueError('clip_grad_norm_: a parameter appears twice')
+    with _on_device(device):
+        stream = stream_ptr()
+        tables = []
+        for dtype, gs in by_type.items():
+            t = (ctypes.c_int64 * (_WORDS * len(gs)))()
+            t[1::_WORDS] = [g.data_ptr() for g in gs]
+            t[6::_WORDS] = [g.numel() for g in gs]
+            tables.append((t, len(gs), dtype_code(dtype)))
+        partials = torch.empty(sum(fn['unetk_grad_partials'](n) for _, n, _ in tables), dtype=torch.float64, device=device)
+        norm = torch.empty((), dtype=torch.float32, device=device)
+        count = 0
+        for t, n, code in tables:
+            count += _written(fn['unetk_grad_sumsq'](ctypes.addressof(t), n, code, partials.data_ptr() + 8 * count, stream),
+                              'unetk_grad_sumsq')
+        if error_if_nonfinite:
+            total = partials[:count].sum().sqrt()
+            if not bool(torch.isfinite(total)):
+                raise RuntimeError('clip_grad_norm_: the norm of the gradients is not finite, so they cannot be clipped')
+        for t, n, code in tables:
+            check(fn['unetk_grad_clip'](ctypes.addressof(t), n, code, partials.data_ptr(), count, max_norm, norm.data_ptr(),
+                                        stream), 'unetk_grad_clip')
+    torch.autograd.graph.increment_version(grads)
+    return norm
+
+
+def _written(count, what):
+    if count < 0:
+        check(int(count), what)
+    return int(count)
+
+
+def dequantize_moment(codes, scales):
+    """fp32 values, in memory order, of 8-bit codes and their block's scales (one column of a state's `scales`)."""
+    x = _memory_order(codes).to(torch.float32)
+    scale = torch.ldexp(torch.ones((), device=x.device), scales.contiguous().view(torch.uint8).to(torch.int32) - 127)
+    return x * scale.repeat_interleave(BLOCK)[:x.numel()]
+
+
+def quantize_moment(x, keep_positive=False):
+    """Codes (to nearest) and scales of fp32 values that lie in one dimension.  `keep_positive`: what is not zero does not
+    become zero, as a root of a second moment must not."""
+    n = x.numel()
+    b = torch.nn.functional.pad(x.detach().to(torch.float32), (0, -n % BLOCK)).view(-1, BLOCK)
+    finite = torch.where(torch.isfinite(b), b, 0.0)
+    frac, power = torch.frexp(finite.abs().amax(1))                 # top = frac * 2^power; 448 = 0.875 * 2^9
+    byte = torch.where(frac > 0, power + (frac > 0.875).to(torch.int32) + 118, 0).clamp(min=0)
+    y = b.double() * torch.exp2(127.0 - byte.double())[:, None]
+    if keep_positive:
+        y = torch.where(y != 0, torch.sign(y) * y.abs().clamp(min=2.0 ** -9), y)
+    y = torch.where(torch.isfinite(y), y, float('nan')).to(torch.float32).to(_CODE)
+    return y.view(-1)[:n], byte.to(torch.uint8).view(_SCALE)
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW over any list of parameters, the whole step in two launches per 64 tensors of one type (include/unetk.h:
+    unetk_adamw_prepare, unetk_adamw_update, unetk_adamw8_update), with clip_grad_norm_(max_norm) over all of them in front.
+
+    params: an iterable of tensors or of parameter groups, on one GPU, in fp32, bf16 or fp16; or a unetk.ddp.FlatGrads, whose
+    flat gradient buffer is then read in place.  Any dense memory layout; a gradient that is laid out unlike its parameter is
+    copied first.
+    max_norm: limit of the 2-norm of all gradients together (one value for all groups), None for no clip.  The gradients
+    themselves stay as they are; `total_norm` holds the norm before the clip (fp32, on the device) after a step.
+    state_bits: 32 keeps `exp_avg` and `exp_avg_sq` in fp32 whatever the parameter's type.  8 keeps them as fp8 codes with a
+    power-of-two scale per 256 elements (2.02 instead of 8 bytes a parameter), rounded stochastically from `seed`, the step and the
+    element's index, for tensors of at least `min_8bit_numel` elements; smaller ones (biases, BatchNorm) keep 32 bits.
+    lr: a float, or an fp32 scalar tensor on the device, which a captured graph reads anew at each replay.
+
+    state[p]: `step` (fp32 scalar on the device), `exp_avg`, and `exp_avg_sq` or, in 8 bits, `exp_avg_root` (the square root)
+    and `scales`.  With 32 bits state_dict() is torch.optim.AdamW's; load_state_dict() takes that one's and either form.
+    Under torch.amp.GradScaler the step is skipped on the device, without a read-back.  A step can be captured into a graph once
+    the state exists (after a first step, or a load_state_dict).
+    """
+    _step_supports_amp_scaling = True
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_norm=None, state_bits=32,
+                 min_8bit_numel=4096, seed=0):
+        self.fg = params if hasattr(params, 'module_order') else None
+        if not isinstance(lr, torch.Tensor) and not lr >= 0:
+            raise ValueError(f'AdamW: lr must not be negative, got {lr}')
+        if not eps >= 0 or not weight_decay >= 0:
+            raise ValueError(f'AdamW: eps and weight_decay must not be negative, got {eps}, {weight_decay}')
+        if state_bits not in (8, 32):
+            raise ValueError(f'AdamW: state_bits must be 8 or 32, got {state_bits}')
+        self.state_bits, self.min_8bit_numel, self.seed = state_bits, int(min_8bit_numel), int(seed) & 0xFFFFFFFF
+        self.total_norm = None
+        if self.fg is not None:          # net.parameters() order, as a stock optimizer numbers its state
+            params = [p for p in self.fg.module_order if id(p) in self.fg.offsets]
+            for p in params:             # laid out like its view of the flat gradients
+                p.data = p.data.contiguous()
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, max_norm=max_norm))
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        try:
+            self._check_group(self.param_groups[-1])
+        except Exception:
+            self.param_groups.pop()
+            raise
+
+    def _check_group(self, g):
+        if len({id(p) for p in g['params']}) != len(g['params']):
+            raise ValueError('AdamW: a parameter appears twice')
+        if not all(0.0 <= b < 1.0 for b in g['betas']):
+            raise ValueError(f"AdamW: betas must lie in [0, 1), got {g['betas']}")
+        if g['max_norm'] is not None and not g['max_norm'] > 0:
+            raise ValueError(f"AdamW: max_norm must be positive or None, got {g['max_norm']}")
+        if g['max_norm'] != self.param_groups[0]['max_norm']:
+            raise ValueError('AdamW: the clip is over all groups: max_norm must be the same in each')
+        for p in g['params']:
+            _require(p, 'parameters')
+            if p.device != next(q for h in self.param_groups for q in h['params']).device:
+                raise RuntimeError('AdamW: parameters must be on one device')
+
+    def zero_grad(self, set_to_none=True):
+        if self.fg is not None:
+            self.fg.consume()
+        super().zero_grad(set_to_none=set_to_none)
+
+    # ---- state
+    def _new_state(self, p):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError('AdamW: take one step (or load a state) before capturing: state made inside a graph would be '
+                               'cleared by every replay')
+        st = {'step': torch.zeros((), dtype=torch.float32, device=p.device)}
+        if self.state_bits == 8 and p.numel() >= self.min_8bit_numel:
+            for k in ('exp_avg', 'exp_avg_root'):
+                st[k] = torch.zeros_like(p, dtype=torch.uint8).view(_CODE)
+            st['scales'] = torch.zeros(-(-p.numel() // BLOCK), 2, dtype=torch.uint8, device=p.device).view(_SCALE)
+        else:
+            for k in ('exp_avg', 'exp_avg_sq'):
+                st[k] = torch.zeros_like(p, dtype=torch.float32)
+        return st
+
+    def _check_state(self, p, st):
+        """The moments lie as the parameter does; moves them if the parameter was laid out anew (net.to(memory_format=...))."""
+        bits = 8 if 'scales' in st else 32
+        names = ('exp_avg', 'exp_avg_root') if bits == 8 else ('exp_avg', 'exp_avg_sq')
+        want = _CODE if bits == 8 else torch.float32
+        for k in names:
+            t = st[k]
+            if t.dtype != want or t.shape != p.shape or t.device != p.device:
+                raise RuntimeError(f'AdamW: state {k!r} must be {want} of shape {tuple(p.shape)} on {p.device}')
+        step = st['step']
+        if not torch.is_tensor(step) or step.dtype != torch.float32 or step.device != p.device or step.numel() != 1:
+            raise RuntimeError("AdamW: state 'step' must be an fp32 scalar on the parameter's device")
+        if bits == 8:
+            sc = st['scales']
+            if sc.dtype != _SCALE or tuple(sc.shape) != (-(-p.numel() // BLOCK), 2) or not sc.is_contiguous() or \
+                    sc.device != p.device:
+                raise RuntimeError("AdamW: state 'scales' must be contiguous float8_e8m0fnu [ceil(numel / 256), 2]")
+        if any(st[k].stride() != p.stride() for k in names):
+            st.update(_fit_moments(p, st, bits))
+        return bits
+
+    # ---- checkpoint / resume.  The file's form (32-bit as torch.optim.AdamW writes it, or 8-bit) need not be this one's.
+    def load_state_dict(self, state_dict):
+        groups = state_dict['param_groups']
+        if [len(g['params']) for g in groups] != [len(g['params']) for g in self.param_groups]:
+            raise ValueError('AdamW.load_state_dict: expected the same parameter groups')
+        for g in groups:
+            if g.get('amsgrad') or g.get('maximize'):
+                raise ValueError('AdamW.load_state_dict: amsgrad and maximize are not implemented')
+        params = [p for g in self.param_groups for p in g['params']]
+        state = {}
+        for index, p in zip([i for g in groups for i in g['params']], params):
+            if index not in state_dict['state']:
+                continue
+            st = state_dict['state'][index]
+            if tuple(st['exp_avg'].shape) != tuple(p.shape):
+                raise ValueError('AdamW.load_state_dict: state shape does not match the parameter')
+            bits = 8 if self.state_bits == 8 and p.numel() >= self.min_8bit_numel else 32
+            state[p] = _fit_moments(p, st, bits)
+            state[p]['step'] = torch.tensor(float(st['step']), dtype=torch.float32, device=p.device)
+        for own, g in zip(self.param_groups, groups):
+            for k in ('lr', 'betas', 'eps', 'weight_decay', 'max_norm', 'initial_lr'):
+                if k in g:
+                    own[k] = g[k]
+        self.state.clear()
+        self.state.update(state)
+
+    # ---- step
+    def _gradient(self, p):
+        return p.grad if self.fg is None else self.fg.views.get(p)
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        if self.fg is not None and self.fg.flat is None:
+            raise RuntimeError('AdamW.step: no gradients (run backward through the UNet first)')
+        jobs, stepped = self._jobs()
+        if stepped:
+            with _on_device(stepped[0].device):
+                self._launch(jobs, stepped[0].device)
+            # the kernels wrote the parameters behind PyTorch's back: bump their version counters like any in-place op
+            torch.autograd.graph.increment_version(stepped)
+        if self.fg is not None:
+            self.fg.consume()
+        return loss
+
+    def _jobs(self):
+        """[(group, type, bits, number of tensors, table, gradients)] and the parameters that take part."""
+        jobs, stepped = [], []
+        for group in self.param_groups:
+            rows = {}
+            for p in group['params']:
+                g = self._gradient(p)
+                if g is None:
+                    continue
+                st = self.state.get(p)
+                if not st:
+                    st = self.state[p] = self._new_state(p)
+                if self.fg is not None and not p.is_contiguous():
+                    p.data = p.data.contiguous()
+                _require(p, 'parameters')
+                bits = self._check_state(p, st)
+                if g.layout != torch.strided or g.dtype != p.dtype or g.device != p.device or g.shape != p.shape:
+                    raise RuntimeError(f'AdamW: a gradient must be a strided tensor of its parameter\'s type, shape and device')
+                if g.stride() != p.stride():
+                    g = torch.empty_like(p).copy_(g)
+                second = st['exp_avg_root' if bits == 8 else 'exp_avg_sq']
+                rows.setdefault((p.dtype, bits), []).append(
+                    (g, (p.data_ptr(), g.data_ptr(), st['exp_avg'].data_ptr(), second.data_ptr(),
+                         st['scales'].data_ptr() if bits == 8 else 0, st['step'].data_ptr(), p.numel())))
+                stepped.append(p)
+            for (dtype, bits), rs in rows.items():
+                table = (ctypes.c_int64 * (_WORDS * len(rs)))(*[w for _, r in rs for w in r])
+                jobs.append((group, dtype_code(dtype), bits, len(rs), table, [g for g, _ in rs]))
+        return jobs, stepped
+
+    def _launch(self, jobs, device):
+        stream = stream_ptr()
+        max_norm = self.param_groups[0]['max_norm']
+        grad_scale, found_inf = getattr(self, 'grad_scale', None), getattr(self, 'found_inf', None)
+        for t in (grad_scale, found_inf):
+            if t is not None and (t.dtype != torch.float32 or t.device != device or t.numel() != 1):
+                raise RuntimeError('AdamW: grad_scale and found_inf must be fp32 scalars on the parameters\' device')
+        scale_ptr = grad_scale.data_ptr() if grad_scale is not None else None
+        found_ptr = found_inf.data_ptr() if found_inf is not None else None
+        # scratch of this call alone, from the allocator of the stream it runs on: calls share none of it
+        sizes = [int(fn['unetk_grad_partials'](n)) if max_norm is not None else 0 for _, _, _, n, _, _ in jobs]
+        tensors = sum(job[3] for job in jobs)
+        scratch = torch.empty(2 * tensors + sum(sizes), dtype=torch.float64, device=device)
+        coefs = scratch.data_ptr()
+        partials = coefs + 16 * tensors if max_norm is not None else None
+        if max_norm is not None:
+            self.total_norm = torch.empty((), dtype=torch.float32, device=device)
+        norm_ptr = self.total_norm.data_ptr() if max_norm is not None else None
+        count, at = 0, coefs
+        for group, code, bits, n, table, _ in jobs:
+            lr, lr_ptr = group['lr'], None
+            if isinstance(lr, torch.Tensor):
+                if lr.is_cuda:
+                    if lr.dtype != torch.float32 or lr.device != device or lr.numel() != 1:
+                        raise RuntimeError('AdamW: a tensor lr must be an fp32 scalar on the parameters\' device')
+                    lr, lr_ptr = 0.0, lr.data_ptr()
+                else:
+                    lr = float(lr)
+            count += _written(fn['unetk_adamw_prepare'](ctypes.addressof(table), n, code, float(lr), lr_ptr, *group['betas'],
+                                                        group['weight_decay'], self.seed, found_ptr, at,
+                                                        partials + 8 * count if partials else None, stream),
+                              'unetk_adamw_prepare')
+            at += 16 * n
+        at = coefs
+        for group, code, bits, n, table, _ in jobs:
+            name = 'unetk_adamw_update' if bits == 32 else 'unetk_adamw8_update'
+            check(fn[name](ctypes.addressof(table), n, code, *group['betas'], group['eps'], scale_ptr, found_ptr, at, partials,
+                           count, max_norm or 0.0, norm_ptr, stream), name)
+            at += 16 * n
+
+
+def _fit_moments(p, st, bits):
+    """The moments of a state in the form and memory layout that parameter `p` needs."""
+    first, second = (torch.empty_like(p, dtype=torch.float32) for _ in range(2))
+    if 'scales' in st:
+        sc = st['scales']
+        for to, k, col in ((first, 'exp_avg', 0), (second, 'exp_avg_root', 1)):
+            x = torch.empty_like(st[k], dtype=torch.float32)
+            _memory_order(x).copy_(dequantize_moment(st[k], sc[:, col]))
+            to.copy_(x)
+    else:
+        first.copy_(st['exp_avg'])
+        second.copy_(st['exp_avg_sq'])
+        if bits == 8:
+            second.sqrt_()
+    if bits == 32:
+        return {'exp_avg': first, 'exp_avg_sq': second.square_() if 'scales' in st else second}
+    out = {}
+    for x, k in ((first, 'exp_avg'), (second, 'exp_avg_root')):
+        codes, sc = quantize_moment(_memory_order(x), keep_positive=k == 'exp_avg_root')
+        out[k] = torch.empty_like(p, dtype=torch.uint8).view(_CODE)
+        _memory_order(out[k].view(torch.uint8)).copy_(codes.view(torch.uint8))
+        out.setdefault('scales', torch.empty(sc.numel(), 2, dtype=torch.uint8, device=p.device).view(_SCALE))
+        out['scales'].view(torch.uint8)[:, 0 if k == 'exp_avg' else 1] = sc.view(torch.uint8)
+    return out

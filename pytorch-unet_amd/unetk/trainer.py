@@ -11,6 +11,11 @@ clip, step (skipped when a gradient overflowed), update.  Clip + RMSprop run as 
 parameter / state buffers (unetk.optim.ClipRMSprop); `fused_optimizer=False` keeps torch's
 foreach RMSprop with the clip applied to the flat gradient buffer (same arithmetic as
 torch.nn.utils.clip_grad_norm_: coef = max_norm / (total_norm + 1e-6), clamped to 1).
+
+optimizer='adamw' steps with unetk.optim.AdamW instead (betas, eps; state_bits=8 keeps its moments in 8 bits): the gradients are
+read where the backward pass left them, `momentum` is not used, and under fp16 a step whose gradients overflowed is skipped on
+the device, without the read-back that 'rmsprop' takes.  fused_optimizer=False then means unetk.optim.clip_grad_norm_ and
+torch.optim.AdamW.
 """
 import torch
 
@@ -21,7 +26,11 @@ from .loss import segmentation_loss
 class Trainer:
     def __init__(self, net, learning_rate=1e-5, weight_decay=1e-8, momentum=0.999, gradient_clipping=1.0, amp=True,
                  process_group=None, bucket_bytes=25 << 20, fused_optimizer=True, force_collectives=False,
-                 amp_dtype=torch.bfloat16):
+                 amp_dtype=torch.bfloat16, optimizer='rmsprop', betas=(0.9, 0.999), eps=1e-8, state_bits=32):
+        if optimizer not in ('rmsprop', 'adamw'):
+            raise ValueError(f"optimizer must be 'rmsprop' or 'adamw', got {optimizer!r}")
+        if state_bits != 32 and not (optimizer == 'adamw' and fused_optimizer):
+            raise ValueError("state_bits other than 32 need optimizer='adamw' with fused_optimizer=True")
         if amp_dtype not in (torch.bfloat16, torch.float16):
             raise ValueError('amp_dtype must be torch.bfloat16 or torch.float16')
         self.net = net
@@ -32,7 +41,15 @@ class Trainer:
         self.clip = gradient_clipping
         self.sync = FlatGrads(net, process_group, bucket_bytes, force_collectives, grads_to_autograd=False)
         self.fused = fused_optimizer
-        if fused_optimizer:
+        self.kind = optimizer
+        if optimizer == 'adamw':
+            from .optim import AdamW
+            kw = dict(lr=learning_rate, betas=betas, eps=eps, weight_decay=weight_decay)
+            if fused_optimizer:
+                self.optimizer = AdamW(self.sync, max_norm=gradient_clipping, state_bits=state_bits, **kw)
+            else:
+                self.optimizer = torch.optim.AdamW(net.parameters(), foreach=True, **kw)
+        elif fused_optimizer:
             from .optim import ClipRMSprop
             self.optimizer = ClipRMSprop(self.sync, lr=learning_rate, weight_decay=weight_decay, momentum=momentum,
                                          max_norm=gradient_clipping)
@@ -59,7 +76,11 @@ class Trainer:
             self.sync.bind_param_grads()
             scaler.unscale_(self.optimizer)
         if not self.fused and flat is not None:
-            if self.clip is not None:
+            if self.clip is not None and self.kind == 'adamw':
+                from .optim import clip_grad_norm_
+                self.sync.bind_param_grads()
+                clip_grad_norm_(self.net.parameters(), self.clip)
+            elif self.clip is not None:
                 total_norm = torch.linalg.vector_norm(flat)
                 flat.mul_(torch.clamp(self.clip / (total_norm + 1e-6), max=1.0))
             # the flat buffer (averaged over ranks, clipped) is authoritative: hand its views to torch's optimizer

@@ -1,0 +1,147 @@
+"""The many-tensor optimizer step without a GPU: what the entry points refuse, and the 8-bit form's helpers."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import adamw_np as O
+
+
+@pytest.fixture(scope='module')
+def nat():
+    from unetk import _native
+    return _native
+
+
+@pytest.fixture(scope='module')
+def optim():
+    from unetk import optim
+    return optim
+
+
+def table(*rows):
+    return (ctypes.c_int64 * (7 * len(rows)))(*[w for r in rows for w in r])
+
+
+ROW = (64, 64, 64, 64, 64, 64, 10)
+
+
+def test_entry_points_refuse_before_launch(nat):
+    fn = nat.fn
+    good, a = table(ROW), ctypes.addressof
+
+    def prepare(t, n=1, dtype=nat.F32, coefs=64, partials=None):
+        return fn['unetk_adamw_prepare'](a(t) if t else None, n, dtype, 1e-3, None, 0.9, 0.999, 0.0, 0, None, coefs, partials, None)
+
+    def update(name, t, n=1, dtype=nat.F32, coefs=64, partials=None, count=0, max_norm=1.0):
+        return fn[name](a(t) if t else None, n, dtype, 0.9, 0.999, 1e-8, None, None, coefs, partials, count, max_norm, None, None)
+
+    assert prepare(None) == -5 and prepare(good, 0) == -5 and prepare(good, dtype=9) == -2 and prepare(good, coefs=None) == -5
+    assert prepare(good, coefs=72) == -3 and prepare(good, partials=12) == -3
+    assert prepare(table(ROW[:5] + (0, 10))) == -5 and prepare(table(ROW[:5] + (66, 10))) == -3      # step
+    assert prepare(table(ROW[:6] + (-1,))) == -5 and prepare(table(ROW[:6] + (1 << 60,))) == -1      # numel
+    for name in ('unetk_adamw_update', 'unetk_adamw8_update'):
+        assert update(name, None) == -5 and update(name, good, -1) == -5 and update(name, good, dtype=3) == -2
+        assert update(name, good, coefs=None) == -5
+        assert update(name, good, partials=64, count=0) == -5 and update(name, good, partials=None, count=4) == -5
+        assert update(name, good, partials=12, count=4) == -3
+        for bad in (-1.0, float('nan')):
+            assert update(name, good, partials=64, count=4, max_norm=bad) == -5
+        for k in range(4):
+            r = list(ROW)
+            r[k] = 0
+            assert update(name, table(r)) == -5
+        r = list(ROW)
+        r[0] = 66                                                       # an fp32 parameter at two bytes
+        assert update(name, table(ROW, r), 2) == -3
+    r = list(ROW)
+    r[4] = 0
+    assert update('unetk_adamw8_update', table(r)) == -5
+    assert fn['unetk_grad_partials'](0) == -5 and fn['unetk_grad_partials'](65) == 2 * fn['unetk_grad_partials'](64)
+    assert fn['unetk_grad_sumsq'](a(good), 1, nat.F32, None, None) == -5
+    assert fn['unetk_grad_sumsq'](a(good), 1, nat.F32, 12, None) == -3
+    assert fn['unetk_grad_clip'](a(good), 1, nat.F32, None, 0, 1.0, None, None) == -5
+    assert fn['unetk_grad_clip'](a(good), 1, nat.BF16, 64, 3, float('nan'), None, None) == -5
+
+
+def test_no_cpu_fallback_and_bad_arguments(optim):
+    p = torch.nn.Parameter(torch.zeros(4))
+    with pytest.raises(RuntimeError, match='cuda'):
+        optim.AdamW([p])
+    p.grad = torch.ones(4)
+    with pytest.raises(RuntimeError, match='cuda'):
+        optim.clip_grad_norm_([p], 1.0)
+    for kw in (dict(lr=-1.0), dict(eps=-1.0), dict(weight_decay=-0.1), dict(state_bits=16), dict(lr=float('nan'))):
+        with pytest.raises(ValueError):
+            optim.AdamW([p], **kw)
+    for kw in (dict(norm_type=1.0), dict(norm_type=float('inf'))):
+        with pytest.raises(ValueError):
+            optim.clip_grad_norm_([p], 1.0, **kw)
+    for bad in (-1.0, float('nan')):
+        with pytest.raises(ValueError):
+            optim.clip_grad_norm_([p], bad)
+    assert float(optim.clip_grad_norm_([torch.nn.Parameter(torch.zeros(2))], 1.0)) == 0.0
+
+
+def test_dense_layouts(optim):
+    t = torch.zeros(3, 4, 5, 6)
+    assert optim._is_dense(t) and optim._is_dense(t.to(memory_format=torch.channels_last)) and optim._is_dense(t.permute(2, 0, 3, 1))
+    assert not optim._is_dense(t[:, :, :, ::2]) and not optim._is_dense(t[:, 1:]) and not optim._is_dense(torch.zeros(1).expand(4))
+    assert optim._is_dense(torch.zeros(0)) and optim._is_dense(torch.zeros(()))
+
+
+@pytest.mark.parametrize('n', [0, 1, 255, 256, 257, 5000])
+def test_moments_to_codes_and_back(optim, n):
+    """Nearest rounding: half of e4m3's step (2^-4 relative, 2^-10 of the scale below its normal range)."""
+    rng = np.random.default_rng(n)
+    x = (rng.standard_normal(n) * 10.0 ** rng.uniform(-12, 3, n)).astype(np.float32)
+    x[: n // 3] *= 1e-30
+    codes, scales = optim.quantize_moment(torch.from_numpy(x))
+    assert codes.dtype == torch.float8_e4m3fn and scales.dtype == torch.float8_e8m0fnu and scales.numel() == -(-n // 256)
+    k = scales.view(torch.uint8).numpy().astype(int) - 127
+    assert np.array_equal(k, O.scale_exponent(x.astype(np.float64)))
+    back = optim.dequantize_moment(codes, scales).numpy().astype(np.float64)
+    unit = np.exp2(np.repeat(k, 256)[:n].astype(float))
+    assert (np.abs(back - x) <= np.abs(x) * 2.0 ** -4 + unit * 2.0 ** -10).all()
+
+
+def test_codes_of_special_values(optim):
+    x = torch.zeros(512)
+    x[0], x[1], x[2], x[3] = float('inf'), float('nan'), 1e-30, 2.0
+    codes, scales = optim.quantize_moment(x, keep_positive=True)
+    back = optim.dequantize_moment(codes, scales)
+    assert torch.isnan(back[:2]).all() and back[3] == 2.0 and 0 < back[2] < 2.0 ** -15 and not back[4:].any()
+    assert int(scales.view(torch.uint8)[1]) == 0
+    codes, _ = optim.quantize_moment(x)
+    assert float(codes[2]) == 0.0
+
+
+@pytest.mark.parametrize('k', [-127, -20, 0, 100])
+def test_the_oracles_rounding_is_unbiased_and_on_the_grid(k):
+    """Averaged over all fractions a code is its value, to the fractions' own 2^-17 of a step; codes are e4m3's."""
+    rng = np.random.default_rng(5)
+    y = rng.uniform(-448, 448, 64) * 10.0 ** -rng.uniform(0, 6, 64)
+    u = (np.arange(65536) + 0.5) / 65536
+    for v in y:
+        q = O.round_code(np.full(65536, v), u, False)
+        assert np.array_equal(q.astype(np.float32), torch.from_numpy(q).float().to(torch.float8_e4m3fn).float().numpy())
+        ulp = np.exp2(max(np.frexp(abs(v))[1] - 4, -9))
+        assert abs(q.mean() - v) <= ulp * 2.0 ** -16
+    x = np.ldexp(y[:1], k)
+    assert O.scale_exponent(np.array([np.ldexp(448.0, k)]))[0] == k and O.scale_exponent(np.array([np.ldexp(448.5, k)]))[0] == k + 1
+    assert O.scale_exponent(x * 0)[0] == -127
+
+
+def test_the_oracles_step_is_torchs():
+    g = torch.Generator().manual_seed(3)
+    p = torch.nn.Parameter(torch.randn(300, generator=g, dtype=torch.float64))
+    opt = torch.optim.AdamW([p], lr=1e-2, betas=(0.9, 0.99), eps=1e-8, weight_decay=0.1)
+    v = dict(p=p.detach().numpy().copy(), m=np.zeros(300), v=np.zeros(300))
+    for t in range(1, 6):
+        p.grad = torch.randn(300, generator=g, dtype=torch.float64)
+        v = O.step(v['p'], p.grad.numpy(), v['m'], v['v'], t, 1e-2, 0.9, 0.99, 1e-8, 0.1)
+        opt.step()
+        assert np.allclose(v['p'], p.detach().numpy(), rtol=1e-12, atol=1e-14)
+    st = opt.state[p]
+    assert np.allclose(st['exp_avg'], v['m'], rtol=1e-12) and np.allclose(st['exp_avg_sq'], v['v'], rtol=1e-12)

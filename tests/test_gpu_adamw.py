@@ -1,0 +1,597 @@
+"""The many-tensor optimizer step (unetk.optim.AdamW, clip_grad_norm_) against its 64-bit restatement, element by element, with
+tolerances counted from the roundings that fp32 arithmetic makes (oracle/adamw_np.py)."""
+import copy
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import adamw_np as O
+
+pytestmark = pytest.mark.gpu
+
+HYPER = dict(lr=1e-2, betas=(0.9, 0.99), eps=1e-8, weight_decay=0.1)
+TYPES = {'fp32': torch.float32, 'bf16': torch.bfloat16, 'fp16': torch.float16}
+COEF_ERR = 6 * O.U                    # of the norm (2), the sum with 1e-6, the quotient, the product with the scale's inverse
+
+
+@pytest.fixture(scope='module')
+def optim():
+    from unetk import optim
+    return optim
+
+
+def f64(t):
+    return t.detach().double().cpu().numpy().ravel()
+
+
+def mem(t):
+    """A dense tensor's values in memory order."""
+    return f64(t.as_strided((t.numel(),), (1,)))
+
+
+def make(sizes, dtype, seed=0, scale=1e-2):
+    g = torch.Generator().manual_seed(seed)
+    out = []
+    for n in sizes:
+        p = torch.nn.Parameter((torch.randn(n, generator=g) * 0.1).to(dtype).cuda())
+        p.grad = (torch.randn(n, generator=g) * scale * 10 ** (2 * torch.rand((), generator=g) - 1)).to(dtype).cuda()
+        out.append(p)
+    return out
+
+
+def snapshot(opt, params):
+    rec = []
+    for p in params:
+        st = opt.state.get(p) or {}
+        r = dict(p=mem(p), g=None if p.grad is None else mem(p.grad), t=float(st['step']) if st else 0.0)
+        n = p.numel()
+        if 'scales' in st:
+            k = st['scales'].view(torch.uint8).cpu().numpy().astype(int) - 127
+            r['k'] = (k[:, 0], k[:, 1])
+            r['codes'] = (mem(st['exp_avg'].float()), mem(st['exp_avg_root'].float()))
+            r['m'], root = (np.ldexp(c, np.repeat(kk, 256)[:n]) for c, kk in zip(r['codes'], r['k']))
+            r['v'] = root ** 2
+        elif st:
+            r['m'], r['v'] = mem(st['exp_avg']), mem(st['exp_avg_sq'])
+        else:
+            r['m'] = r['v'] = np.zeros(n)
+        rec.append(r)
+    return rec
+
+
+def check_step(params, before, after, hyper, max_norm=None, seed=0, total_norm=None, grad_scale=1.0):
+    grads = [b['g'] / grad_scale for b in before if b['g'] is not None]
+    factor, err = 1.0 / grad_scale, 0.0
+    if max_norm is not None:
+        norm = O.norm(grads)
+        assert abs(float(total_norm) - norm) <= 3 * O.U * norm
+        factor, err = O.clip_coef(norm, max_norm) / grad_scale, COEF_ERR
+    for p, b, a in zip(params, before, after):
+        if b['g'] is None:
+            assert a['t'] == b['t'] and np.array_equal(a['p'], b['p'])
+            continue
+        t = b['t'] + 1
+        assert a['t'] == t
+        fi = torch.finfo(p.dtype)
+        half, tiny = (0.0, 0.0) if p.dtype == torch.float32 else (fi.eps / 2, fi.smallest_normal)
+        want = O.step(b['p'], b['g'], b['m'], b['v'], t, hyper['lr'], *hyper['betas'], hyper['eps'], hyper['weight_decay'],
+                      factor, err, half, tiny)
+        assert (np.abs(a['p'] - want['p']) <= want['pe']).all(), np.abs(a['p'] - want['p']).max()
+        if 'k' not in a:
+            assert (np.abs(a['m'] - want['m']) <= want['me']).all()
+            assert (np.abs(a['v'] - want['v']) <= want['ve']).all()
+            continue
+        for x, xe, k, codes, u, root in zip((want['m'], want['r']), (want['me'], want['re']), a['k'], a['codes'],
+                                            O.fractions(len(b['p']), t, seed), (False, True)):
+            for kk, lo, hi in zip(k, O.scale_exponent(np.maximum(np.abs(x) - xe, 0)), O.scale_exponent(np.abs(x) + xe)):
+                assert lo <= kk <= hi
+            lo, hi = O.code_range(x, xe, k, u, root)
+            assert (lo <= codes).all() and (codes <= hi).all()
+            assert (lo == hi).mean() > 0.99 or len(lo) < 1000       # the bound leaves a choice at almost no element
+
+
+SIZES = {'one': [1], 'small': [3, 1, 2, 255, 256, 257], 'edges': [4095, 4096, 4097, 8191, 12288 + 1], 'mixed': [100003, 7, 4096, 65537, 64],
+         'many': [1 + (37 * i) % 700 for i in range(64)], 'more': [1 + (53 * i) % 500 for i in range(65)],
+         'lots': [1 + (29 * i) % 300 for i in range(200)]}
+
+
+@pytest.mark.parametrize('sizes', list(SIZES))
+@pytest.mark.parametrize('bits', [32, 8])
+@pytest.mark.parametrize('dtype', list(TYPES))
+@pytest.mark.parametrize('max_norm', [None, 0.5])
+def test_steps(optim, sizes, bits, dtype, max_norm):
+    params = make(SIZES[sizes], TYPES[dtype], seed=len(sizes))
+    opt = optim.AdamW(params, **HYPER, max_norm=max_norm, state_bits=bits, min_8bit_numel=1, seed=77)
+    for k in range(3):
+        before = snapshot(opt, params)
+        opt.step()
+        after = snapshot(opt, params)
+        check_step(params, before, after, HYPER, max_norm, 77, opt.total_norm)
+        assert all(np.array_equal(b['g'], a['g']) for a, b in zip(after, before))      # gradients stay as they are
+        for i, p in enumerate(params):
+            p.grad = torch.randn_like(p) * 10.0 ** (-2 - (i + k) % 3)
+
+
+@pytest.mark.parametrize('bits', [32, 8])
+def test_no_limit_reached_and_extreme_hyperparameters(optim, bits):
+    """A limit above the norm changes nothing; beta 0, weight decay 0, eps 0 and lr 0 are what the formula says."""
+    for hyper, max_norm in ((HYPER, 1e6), (dict(lr=1e-3, betas=(0.0, 0.9), eps=1e-3, weight_decay=0.0), 1e6),
+                            (dict(lr=0.0, betas=(0.9, 0.0), eps=1e-8, weight_decay=0.0), None)):
+        a, b = make([5000, 33], torch.float32), make([5000, 33], torch.float32)
+        oa = optim.AdamW(a, **hyper, max_norm=max_norm, state_bits=bits, min_8bit_numel=1)
+        ob = optim.AdamW(b, **hyper, state_bits=bits, min_8bit_numel=1)
+        for _ in range(2):
+            before = snapshot(oa, a)
+            oa.step(), ob.step()
+            check_step(a, before, snapshot(oa, a), hyper, max_norm, 0, oa.total_norm)
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+        if hyper['lr'] == 0.0:
+            assert all(torch.equal(x, y) for x, y in zip(a, make([5000, 33], torch.float32)))
+
+
+@pytest.mark.parametrize('dtype', list(TYPES))
+@pytest.mark.parametrize('bits', [32, 8])
+@pytest.mark.parametrize('shift', [1, 3])
+def test_views_at_any_address_touch_nothing_else(optim, dtype, bits, shift):
+    """Tensors that lie one behind the other at odd elements of one buffer, with a guard in front, between and behind."""
+    dt, sizes, gap = TYPES[dtype], [1, 257, 4096, 4099, 31, 70001], 5
+    off, starts = shift, []
+    for n in sizes:
+        starts.append(off)
+        off += n + gap
+    g = torch.Generator().manual_seed(1)
+
+    def buffer(d):
+        raw = torch.randn(off + 8, generator=g).cuda()
+        return raw.to(d) if d.itemsize > 1 else (raw.abs() * 8).to(d)
+
+    bufs = {k: buffer(d) for k, d in (('p', dt), ('g', dt), ('m', torch.float32 if bits == 32 else torch.float8_e4m3fn),
+                                      ('v', torch.float32 if bits == 32 else torch.float8_e4m3fn))}
+    if bits == 32:
+        bufs['v'].abs_()
+    saved = {k: v.clone() for k, v in bufs.items()}
+    views = {k: [b[a:a + n] for a, n in zip(starts, sizes)] for k, b in bufs.items()}
+    params = [torch.nn.Parameter(p) for p in views['p']]
+    opt = optim.AdamW(params, **HYPER, max_norm=1.0, state_bits=bits, min_8bit_numel=1)
+    for i, (p, n) in enumerate(zip(params, sizes)):
+        p.grad = views['g'][i]
+        opt.state[p] = {'step': torch.full((), 4.0, device='cuda'), 'exp_avg': views['m'][i],
+                        ('exp_avg_sq' if bits == 32 else 'exp_avg_root'): views['v'][i]}
+        if bits == 8:
+            scales = torch.full((2 * -(-n // 256) + 1,), 125, dtype=torch.uint8, device='cuda')[i % 2:][:2 * -(-n // 256)]
+            opt.state[p]['scales'] = scales.view(-1, 2).view(torch.float8_e8m0fnu)          # at an odd address, too
+    before = snapshot(opt, params)
+    opt.step()
+    check_step(params, before, snapshot(opt, params), HYPER, 1.0, 0, opt.total_norm)
+    inside = torch.zeros(off + 8, dtype=torch.bool)
+    for a, n in zip(starts, sizes):
+        inside[a:a + n] = True
+    for k, b in bufs.items():
+        raw = torch.uint8 if b.element_size() == 1 else torch.int16 if b.element_size() == 2 else torch.int32
+        same = (b.view(raw) == saved[k].view(raw)).cpu()
+        assert same[~inside].all(), k
+        assert k != 'g' or same.all()
+
+
+def test_empty_tensors_missing_gradients_and_own_step_counts(optim):
+    params = make([10, 0, 5000, 7, 0], torch.float32)
+    opt = optim.AdamW(params, **HYPER, max_norm=1.0, state_bits=8)
+    for k in range(4):
+        params[2].grad = None if k == 1 else torch.randn_like(params[2])
+        before = snapshot(opt, params)
+        opt.step()
+        check_step(params, before, snapshot(opt, params), HYPER, 1.0, 0, opt.total_norm)
+    assert float(opt.state[params[2]]['step']) == 3.0 and float(opt.state[params[0]]['step']) == 4.0
+    assert 'scales' in opt.state[params[2]] and 'scales' not in opt.state[params[0]]
+    for p in params:
+        p.grad = None
+    before = snapshot(opt, params)
+    opt.step()
+    assert all(np.array_equal(a['p'], b['p']) for a, b in zip(snapshot(opt, params), before))
+
+
+@pytest.mark.parametrize('bits', [32, 8])
+def test_values_that_are_not_finite_stay_where_they_are(optim, bits):
+    """Without a clip one element's infinity or NaN is that element's alone; an 8-bit block keeps the others' codes."""
+    clean, dirty = make([3000], torch.float32), make([3000], torch.float32)
+    dirty[0].grad[5], dirty[0].grad[300], dirty[0].grad[301] = float('nan'), float('inf'), -float('inf')
+    opts = [optim.AdamW(p, **HYPER, state_bits=bits, min_8bit_numel=1) for p in (clean, dirty)]
+    for p in (clean, dirty):
+        p[0].grad[7] = 0.0
+    for _ in range(2):
+        for o in opts:
+            o.step()
+    bad = torch.zeros(3000, dtype=torch.bool)
+    bad[[5, 300, 301]] = True
+    (sa, sb), k2 = (o.state[p[0]] for o, p in zip(opts, (clean, dirty))), 'exp_avg_sq' if bits == 32 else 'exp_avg_root'
+    for x, y in [(clean[0], dirty[0])] + [(sa[k], sb[k]) for k in ('exp_avg', k2)]:
+        x, y = x.detach().float().cpu(), y.detach().float().cpu()
+        if x.shape == (3000,):
+            assert not torch.isfinite(y[bad]).any()
+        keep = ~bad
+        if bits == 8:                                # the bad elements may have held a block's largest value
+            keep[:512] = False
+            assert torch.isfinite(y[:512][~bad[:512]]).all()
+        assert torch.equal(x[keep], y[keep])
+
+
+def test_a_norm_that_is_not_finite_spreads_as_torchs_does(optim):
+    for bad in (float('nan'), float('inf')):
+        p = make([40, 600], torch.float32)
+        p[0].grad[3] = bad
+        q = [torch.nn.Parameter(x.detach().clone()) for x in p]
+        for x, y in zip(p, q):
+            y.grad = x.grad.clone()
+        want = torch.nn.utils.clip_grad_norm_(q, 1.0)
+        got = optim.clip_grad_norm_(p, 1.0)
+        assert torch.equal(torch.isnan(want), torch.isnan(got)) and torch.equal(torch.isinf(want), torch.isinf(got))
+        for x, y in zip(p, q):
+            assert torch.equal(torch.isnan(x.grad), torch.isnan(y.grad))
+        p[0].grad[3] = bad
+        with pytest.raises(RuntimeError, match='not finite'):
+            optim.clip_grad_norm_(p, 1.0, error_if_nonfinite=True)
+
+
+def test_8bit_rounding_does_not_freeze_the_second_moment(optim):
+    """With no gradient the root decays by sqrt(b2) a step; rounding to nearest would leave it where it is.  A step moves r by
+    0.5 % where codes lie r / 16 apart at least, so it changes a code with probability p <= 0.08 and adds a variance of at most
+    0.074 ulp^2, ulp <= 0.1 / 8: over 100 steps and 65536 elements the mean deviates by 1.3e-4, 0.22 % of it."""
+    n, steps, b2 = 65536, 100, 0.99
+    p = torch.nn.Parameter(torch.zeros(n, device='cuda'))
+    p.grad = torch.full_like(p, 1.0)
+    opt = optim.AdamW([p], lr=0.0, betas=(0.9, b2), state_bits=8)
+    opt.step()
+    p.grad = torch.zeros_like(p)
+    for _ in range(steps):
+        opt.step()
+    st = opt.state[p]
+    root = optim.dequantize_moment(st['exp_avg_root'], st['scales'][:, 1])
+    want = math.sqrt((1 - b2) * b2 ** steps)
+    assert abs(float(root.mean()) / want - 1) < 0.015
+    assert float(root.min()) > 0
+
+
+# ------------------------------------------------------------------------------------------ layouts, streams, graphs
+@pytest.mark.parametrize('bits', [32, 8])
+def test_channels_last_parameters_and_a_change_of_layout(optim, bits):
+    g = torch.Generator().manual_seed(4)
+    w = torch.randn(24, 40, 3, 3, generator=g)
+    grads = [torch.randn(24, 40, 3, 3, generator=g) for _ in range(3)]
+    a = torch.nn.Parameter(w.cuda())
+    b = torch.nn.Parameter(w.cuda().to(memory_format=torch.channels_last))
+    oa, ob = (optim.AdamW([p], **HYPER, state_bits=bits, min_8bit_numel=1) for p in (a, b))
+    for k, gr in enumerate(grads):
+        a.grad = gr.cuda()
+        b.grad = gr.cuda() if k != 1 else gr.cuda().to(memory_format=torch.channels_last)     # like its parameter, or not
+        if k == 2:                                                                            # net.to(memory_format=...) later
+            a.data = a.data.to(memory_format=torch.channels_last)
+            b.data = b.data.contiguous()
+        before = snapshot(ob, [b])
+        if k < 2:
+            before[0]['g'] = mem(torch.empty_like(b).copy_(b.grad))
+            oa.step(), ob.step()
+            check_step([b], before, snapshot(ob, [b]), HYPER)
+        else:
+            oa.step(), ob.step()
+    assert ob.state[b]['exp_avg'].stride() == b.stride()
+    if bits == 32:
+        assert torch.equal(a, b) and torch.equal(oa.state[a]['exp_avg'], ob.state[b]['exp_avg'])
+    else:
+        # the third step starts from moments that were rounded to nearest in another order's blocks: 2^-4 of each, and a
+        # sixteenth of m and of the root moves a step of at most lr * 2.4 (three steps, b2 = 0.99) by less than an eighth, twice
+        assert float((a.detach() - b.detach()).abs().max()) <= 3 * 2 * HYPER['lr'] * 2.4
+
+
+def test_another_stream(optim):
+    params, twin = make([200001, 50], torch.float32), make([200001, 50], torch.float32)
+    opt, ref = (optim.AdamW(p, **HYPER, max_norm=0.1, state_bits=8) for p in (params, twin))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(5):
+            opt.step()
+            optim.clip_grad_norm_(params, 1e9)
+    torch.cuda.current_stream().wait_stream(s)
+    for _ in range(5):
+        ref.step()
+    assert all(torch.equal(a, b) for a, b in zip(params, twin)) and torch.equal(opt.total_norm, ref.total_norm)
+
+
+@pytest.mark.parametrize('bits', [32, 8])
+def test_a_captured_step_counts_and_follows_the_learning_rate(optim, bits):
+    sizes = [70001, 300, 5]
+    params, twin = make(sizes, torch.float32), make(sizes, torch.float32)
+    lr = torch.tensor(1e-2, device='cuda')
+    kw = dict(HYPER, max_norm=0.2, state_bits=bits, seed=5)
+    opt, ref = optim.AdamW(params, **dict(kw, lr=lr)), optim.AdamW(twin, **kw)
+    with pytest.raises(RuntimeError, match='before capturing'):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    opt.step(), ref.step()
+    graph, scratch = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    norm = opt.total_norm
+    with torch.cuda.graph(scratch):                                   # another graph's scratch is its own
+        optim.clip_grad_norm_(twin, 1e9)
+    for k in range(4):
+        rate = 1e-2 / (k + 1)
+        lr.fill_(rate)
+        ref.param_groups[0]['lr'] = float(lr)
+        for p, q in zip(params, twin):
+            new = torch.randn_like(p) * 10.0 ** -k
+            p.grad.copy_(new), q.grad.copy_(new)
+        graph.replay()
+        ref.step()
+        scratch.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(params, twin)), k
+        assert torch.equal(norm, ref.total_norm)
+        assert float(opt.state[params[0]]['step']) == float(ref.state[twin[0]]['step']) == k + 2
+    for p, q in zip(params, twin):
+        for key, x in opt.state[p].items():
+            y = ref.state[q][key]
+            assert torch.equal(x.view(torch.uint8), y.view(torch.uint8)) if x.element_size() == 1 else torch.equal(x, y)
+
+
+def test_grad_scaler_skips_on_the_device(optim):
+    params, twin = make([5000, 40], torch.float32), make([5000, 40], torch.float32)
+    opt, ref = optim.AdamW(params, **HYPER, max_norm=0.1), optim.AdamW(twin, **HYPER, max_norm=0.1)
+    scaler = torch.amp.GradScaler('cuda', init_scale=1024.0)
+    scaler.scale(torch.zeros((), device='cuda'))
+    for k, (overflow, unscale) in enumerate([(False, False), (True, False), (False, True), (True, True), (False, False)]):
+        for p, q in zip(params, twin):
+            new = torch.randn_like(p)
+            p.grad, q.grad = new * float(scaler.get_scale()), new.clone()
+        if overflow:
+            params[1].grad[3] = float('inf')
+        if unscale:
+            scaler.unscale_(opt)
+        kept = [p.detach().clone() for p in params]
+        scaler.step(opt)
+        scaler.update()
+        if overflow:
+            assert all(torch.equal(p, q) for p, q in zip(params, kept))
+        else:
+            ref.step()
+            assert all(torch.equal(p, q) for p, q in zip(params, twin)), k      # the scales are powers of two
+    assert float(opt.state[params[0]]['step']) == 3.0
+    assert not hasattr(opt, 'found_inf')
+
+
+def test_two_optimizers_take_turns(optim):
+    """Scratch belongs to a call: interleaved steps of two optimizers give what each gives alone."""
+    def one():
+        p = make([30001, 77], torch.float32, seed=8)
+        return p, optim.AdamW(p, **HYPER, max_norm=0.3, state_bits=8)
+    a, b, c = one(), one(), one()
+    for _ in range(3):
+        a[1].step(), b[1].step()
+    for _ in range(3):
+        c[1].step()
+    for x in (a, b):
+        assert all(torch.equal(p, q) for p, q in zip(x[0], c[0]))
+
+
+# ---------------------------------------------------------------------------------------------------- checkpoints
+def test_32bit_checkpoints_are_torchs(optim):
+    a, b, c = (make([300, 4097], torch.float32) for _ in range(3))
+    kw = dict(HYPER)
+    ours, stock, third = optim.AdamW(a, **kw), torch.optim.AdamW(b, **kw), optim.AdamW(c, **dict(kw, lr=5.0))
+    for _ in range(2):
+        ours.step(), stock.step()
+    for p, q in zip(a, b):
+        assert torch.allclose(p, q, rtol=1e-5, atol=1e-7)
+    sd = ours.state_dict()
+    assert set(sd['state'][0]) == {'step', 'exp_avg', 'exp_avg_sq'}
+    b2 = [torch.nn.Parameter(p.detach().clone()) for p in a]
+    stock2 = torch.optim.AdamW(b2, **kw)
+    stock2.load_state_dict(copy.deepcopy({**sd, 'param_groups': [{**stock2.state_dict()['param_groups'][0]}]}))
+    for p, q in zip(c, a):
+        p.data.copy_(q.data)
+    third.load_state_dict(stock2.state_dict())
+    assert third.param_groups[0]['lr'] == kw['lr'] and third.state[c[0]]['step'].is_cuda
+    for p, q, r in zip(b2, a, c):
+        p.grad = q.grad = r.grad = torch.randn_like(q)
+    ours.step(), stock2.step(), third.step()
+    for p, q, r in zip(a, b2, c):
+        assert torch.allclose(p, q, rtol=1e-5, atol=1e-7) and torch.equal(p, r)
+    bad = copy.deepcopy(sd)
+    bad['state'][0]['exp_avg'] = torch.zeros(299)
+    with pytest.raises(ValueError, match='shape'):
+        third.load_state_dict(bad)
+    bad = copy.deepcopy(sd)
+    bad['param_groups'][0]['amsgrad'] = True
+    with pytest.raises(ValueError, match='amsgrad'):
+        third.load_state_dict(bad)
+    with pytest.raises(ValueError, match='groups'):
+        optim.AdamW(c[:1], **kw).load_state_dict(sd)
+
+
+def test_8bit_checkpoints_resume_to_the_bit_and_convert(optim, tmp_path):
+    a, b = make([300, 70001], torch.bfloat16), make([300, 70001], torch.bfloat16)
+    oa, ob = (optim.AdamW(p, **HYPER, state_bits=8, seed=3) for p in (a, b))
+    for _ in range(3):
+        oa.step()
+    torch.save(oa.state_dict(), tmp_path / 'opt.pth')
+    sd = torch.load(tmp_path / 'opt.pth', weights_only=True)
+    for p, q in zip(b, a):
+        p.data.copy_(q.data)
+    ob.load_state_dict(sd)
+    # into 32 bits: exactly what the codes stand for
+    c = [torch.nn.Parameter(p.detach().clone()) for p in a]
+    oc = optim.AdamW(c, **HYPER)
+    oc.load_state_dict(sd)
+    st = oa.state[a[1]]
+    assert torch.equal(oc.state[c[1]]['exp_avg'], optim.dequantize_moment(st['exp_avg'], st['scales'][:, 0]))
+    assert torch.equal(oc.state[c[1]]['exp_avg_sq'], optim.dequantize_moment(st['exp_avg_root'], st['scales'][:, 1]) ** 2)
+    # and from 32 bits into 8: half a step of e4m3 (2^-4, 2^-10 of the scale among its subnormals)
+    od = optim.AdamW([torch.nn.Parameter(p.detach().clone()) for p in a], **HYPER, state_bits=8)
+    od.load_state_dict(oc.state_dict())
+    sd2 = od.state[od.param_groups[0]['params'][1]]
+    for k, col, ref in (('exp_avg', 0, oc.state[c[1]]['exp_avg']), ('exp_avg_root', 1, oc.state[c[1]]['exp_avg_sq'].sqrt())):
+        unit = optim.dequantize_moment(torch.ones(70001, device='cuda').to(torch.float8_e4m3fn), sd2['scales'][:, col])
+        assert ((optim.dequantize_moment(sd2[k], sd2['scales'][:, col]) - ref).abs() <= ref.abs() * 2.0 ** -4 + unit * 2.0 ** -9).all()
+    oa.step(), ob.step()
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    for k in ('exp_avg', 'exp_avg_root', 'scales'):
+        assert torch.equal(oa.state[a[1]][k].view(torch.uint8), ob.state[b[1]][k].view(torch.uint8))
+
+
+# --------------------------------------------------------------------------------------------------------- refusals
+def test_refusals(optim):
+    p = make([10, 20], torch.float32)
+    with pytest.raises(ValueError, match='twice'):
+        optim.AdamW([{'params': [p[0], p[0]]}])
+    for kw in (dict(betas=(1.0, 0.9)), dict(betas=(0.9, -0.1)), dict(max_norm=0.0), dict(max_norm=-1.0)):
+        with pytest.raises(ValueError):
+            optim.AdamW(p, **kw)
+    with pytest.raises(ValueError, match='same in each'):
+        optim.AdamW([{'params': [p[0]], 'max_norm': 1.0}, {'params': [p[1]], 'max_norm': 2.0}])
+    with pytest.raises(RuntimeError, match='float64'):
+        optim.AdamW([torch.nn.Parameter(torch.zeros(3, dtype=torch.float64, device='cuda'))])
+    with pytest.raises(RuntimeError, match='dense'):
+        optim.AdamW([torch.nn.Parameter(torch.zeros(8, 8, device='cuda')[:, ::2])])
+    opt = optim.AdamW(p)
+    with pytest.raises(ValueError):
+        opt.add_param_group({'params': [torch.nn.Parameter(torch.zeros(1, device='cuda'))], 'betas': (2.0, 0.1)})
+    assert len(opt.param_groups) == 1
+    opt.step()
+    for key, value in (('step', torch.zeros(())), ('exp_avg', torch.zeros(10, device='cuda', dtype=torch.bfloat16)),
+                       ('exp_avg_sq', torch.zeros(9, device='cuda'))):
+        old, opt.state[p[0]][key] = opt.state[p[0]][key], value
+        with pytest.raises(RuntimeError, match=key):
+            opt.step()
+        opt.state[p[0]][key] = old
+    e = torch.nn.Parameter(torch.zeros(4, device='cuda'))
+    e.grad = torch.zeros(1, device='cuda').expand(4)
+    with pytest.raises(RuntimeError, match='dense'):
+        optim.clip_grad_norm_([e], 1.0)
+    with pytest.raises(ValueError, match='twice'):
+        optim.clip_grad_norm_([p[0], p[0]], 1.0)
+    opt.param_groups[0]['lr'] = torch.tensor(1e-3, dtype=torch.float64, device='cuda')
+    with pytest.raises(RuntimeError, match='lr'):
+        opt.step()
+
+
+# ------------------------------------------------------------------------------------------------------------- clip
+@pytest.mark.parametrize('sizes', list(SIZES))
+@pytest.mark.parametrize('dtype', list(TYPES) + ['mixed'])
+def test_clip_grad_norm(optim, sizes, dtype):
+    if dtype == 'mixed':
+        params = [q for i, n in enumerate(SIZES[sizes]) for q in make([n], list(TYPES.values())[i % 3], seed=i)]
+    else:
+        params = make(SIZES[sizes], TYPES[dtype])
+    before = [mem(p.grad) for p in params]
+    norm = O.norm(before)
+    for limit in (norm * 0.37, norm * 2, math.inf, 0.0):
+        for p, b in zip(params, before):
+            p.grad.copy_(torch.from_numpy(b).to(p.dtype))
+        got = optim.clip_grad_norm_(params, limit)
+        assert got.dtype == torch.float32 and got.is_cuda and abs(float(got) - norm) <= 3 * O.U * norm
+        c = O.clip_coef(norm, limit)
+        for p, b in zip(params, before):
+            fi = torch.finfo(p.dtype)
+            err = np.abs(b * c) * (COEF_ERR + O.U + fi.eps / 2) + fi.eps / 2 * fi.smallest_normal
+            assert (np.abs(mem(p.grad) - b * c) <= (err if c < 1 else 0)).all()
+
+
+def test_clip_of_huge_and_tiny_gradients(optim):
+    """Squares beyond fp32's range: the norm is still the norm."""
+    for value in (1e30, 1e-30):
+        p = torch.nn.Parameter(torch.zeros(1000, device='cuda'))
+        p.grad = torch.full_like(p, value)
+        got = float(optim.clip_grad_norm_([p], value))
+        want = float(np.float32(value)) * math.sqrt(1000)
+        assert abs(got - want) <= 3 * O.U * want
+
+
+def test_more_than_two_to_the_31_elements(optim):
+    """Offsets beyond 32 bits: the last elements of a tensor of 2^31 + 4099."""
+    n, tail = 2 ** 31 + 4099, 5000
+    p = torch.nn.Parameter(torch.zeros(n, dtype=torch.bfloat16, device='cuda'))
+    p.grad = torch.zeros(n, dtype=torch.bfloat16, device='cuda')
+    g = torch.randn(tail, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16)
+    p.grad[-tail:] = g.cuda()
+    opt = optim.AdamW([p], **HYPER, state_bits=8, max_norm=1.0, seed=9)
+    opt.step()
+    want_norm = O.norm([f64(g)])
+    assert abs(float(opt.total_norm) - want_norm) <= 3 * O.U * want_norm
+    c = O.clip_coef(want_norm, 1.0)
+    fi = torch.finfo(torch.bfloat16)
+    want = O.step(np.zeros(tail), f64(g), np.zeros(tail), np.zeros(tail), 1, HYPER['lr'], *HYPER['betas'], 1e-8, 0.1, c, COEF_ERR,
+                  fi.eps / 2, fi.smallest_normal)
+    assert (np.abs(f64(p[-tail:]) - want['p']) <= want['pe']).all()
+    assert not p[:-tail].any()
+    st = opt.state[p]
+    first = (n - tail) // 256 * 256                                   # whole blocks from here
+    lead = n - tail - first
+    k = st['scales'].view(torch.uint8)[first // 256:].cpu().numpy().astype(int) - 127
+    for key, col, x, xe, u in (('exp_avg', 0, want['m'], want['me'], O.fractions(n - first, 1, 9, first)[0]),
+                               ('exp_avg_root', 1, want['r'], want['re'], O.fractions(n - first, 1, 9, first)[1])):
+        x, xe = (np.concatenate([np.zeros(lead), y]) for y in (x, xe))
+        xe[:lead] = 0
+        lo, hi = O.code_range(x, xe, k[:, col], u, col == 1)
+        codes = f64(st[key][first:].float())
+        assert (lo <= codes).all() and (codes <= hi).all()
+
+
+# ------------------------------------------------------------------------------------------------------- the trainer
+def test_the_trainer_steps_with_it(optim):
+    """Trainer(optimizer='adamw') on the flat gradient buffer against torch.optim.AdamW fed with the same gradients; 8 bits
+    moves the same way; the checkpoint is numbered in net.parameters() order."""
+    from test_gpu_trainstep import _closed_form, _img, SHAPE
+    from unet import UNet
+    from unetk.trainer import Trainer
+    img = _img()
+    mask = (torch.arange(SHAPE[0] * SHAPE[2] * SHAPE[3], device='cuda') % 7 == 0).long().view(SHAPE[0], SHAPE[2], SHAPE[3])
+    net = _closed_form(UNet(3, 2, False)).cuda().to(memory_format=torch.channels_last).train()
+    twin = [torch.nn.Parameter(p.detach().clone().contiguous()) for p in net.parameters()]
+    tr = Trainer(net, amp=False, learning_rate=1e-4, weight_decay=0.01, optimizer='adamw')
+    stock = torch.optim.AdamW(twin, lr=1e-4, weight_decay=0.01)
+    for _ in range(2):
+        tr.step(img, mask)
+        for p, q in zip(net.parameters(), twin):
+            q.grad = tr.sync.views[p].detach().clone()
+        norm = torch.nn.utils.clip_grad_norm_(twin, 1.0)
+        assert abs(float(norm) - float(tr.optimizer.total_norm)) <= 1e-5 * float(norm)
+        stock.step()
+        for p, q in zip(net.parameters(), twin):
+            # the same gradients: the decay, the difference and the store round a parameter three times on each side and step, and
+            # a step of at most lr / (1 - beta1) carries the moments' roundings, some 10 of 2^-24
+            assert ((p - q).abs() <= 12 * 2.0 ** -24 * q.abs() + 2 * 20 * 2.0 ** -24 * 1e-3).all()
+    sd = tr.optimizer.state_dict()
+    for i, q in enumerate(twin):
+        assert sd['state'][i]['exp_avg'].shape == q.shape
+    for kw in (dict(optimizer='sgd'), dict(state_bits=8), dict(optimizer='adamw', state_bits=8, fused_optimizer=False)):
+        with pytest.raises(ValueError, match='optimizer'):
+            Trainer(net, **kw)
+    # the same loop around a stock optimizer, with the clip by itself
+    net2 = _closed_form(UNet(3, 2, False)).cuda().to(memory_format=torch.channels_last).train()
+    tr2 = Trainer(net2, amp=False, learning_rate=1e-4, weight_decay=0.01, optimizer='adamw', fused_optimizer=False)
+    tr2.step(img, mask)
+    total = sum(float(p.grad.double().square().sum()) for p in net2.parameters()) ** 0.5
+    assert total <= 1.0 + 1e-5 and type(tr2.optimizer) is torch.optim.AdamW
+
+
+@pytest.mark.parametrize('amp_dtype', [torch.bfloat16, torch.float16])
+def test_the_trainer_in_mixed_precision_with_8bit_moments(optim, amp_dtype):
+    from test_gpu_trainstep import _closed_form, _img, SHAPE
+    from unet import UNet
+    from unetk.trainer import Trainer
+    img = _img()
+    mask = (torch.arange(SHAPE[0] * SHAPE[2] * SHAPE[3], device='cuda') % 7 == 0).long().view(SHAPE[0], SHAPE[2], SHAPE[3])
+    net = _closed_form(UNet(3, 2, False)).cuda().to(memory_format=torch.channels_last).train()
+    tr = Trainer(net, learning_rate=1e-4, weight_decay=0.01, optimizer='adamw', state_bits=8, amp_dtype=amp_dtype)
+    for k in range(2):
+        before = snapshot(tr.optimizer, list(net.parameters()))
+        tr.step(img, mask)
+        params = list(net.parameters())
+        for b, p in zip(before, params):
+            b['g'] = f64(tr.sync.views[p])
+        check_step(params, before, snapshot(tr.optimizer, params), dict(lr=1e-4, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01),
+                   1.0, 0, tr.optimizer.total_norm)
+    kinds = {'scales' in tr.optimizer.state[p] for p in net.parameters()}
+    assert kinds == {True, False}
