@@ -355,9 +355,9 @@ int unetk_clip_rmsprop_step(float* param, float* grad, float* square_avg, float*
  * tensors need not lie in one buffer, may have any number of elements (0 included) and any element-aligned address.
  * No reference counterpart: the reference trains with RMSprop (train.py:77-78); the clip is its train.py:115.
  *
- * `tensors` is a HOST array that is read during the call (its contents travel as kernel arguments, so a captured graph
- * replays the pointers it was captured with).  A call serves tensors of one element type (`dtype`: parameter and
- * gradient); elements are taken in memory order, so all arrays of a tensor share one dense layout.
+ * `tensors`, `grads` (and `numel`) are HOST arrays of n_tensors entries that are read during the call; their contents travel as
+ * kernel arguments, so a captured graph replays the pointers it was captured with.  A call serves tensors of one element type
+ * (`dtype`: parameter and gradient); elements are taken in memory order, so all arrays of a tensor share one dense layout.
  *   coef = min(1, max_norm / (norm + 1e-6)), norm = sqrt(sum of the partials) / grad_scale   (no partials: coef = 1)
  *   g = coef * grad / grad_scale;  step += 1;  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2
  *   param = param (1 - lr wd) - lr / (1 - b1^step) * m / (sqrt(v) / sqrt(1 - b2^step) + eps)
@@ -384,10 +384,9 @@ int unetk_clip_rmsprop_step(float* param, float* grad, float* square_avg, float*
  * grad_scale, found_inf (device, may be NULL): torch.amp.GradScaler's; found_inf != 0 skips the step, its count included.
  *
  * unetk_grad_sumsq + unetk_grad_clip: torch.nn.utils.clip_grad_norm_ (reference train.py:115) by themselves, gradients
- * scaled in place (not written where coef is 1); they read `grad` and `numel` of the records only. */
+ * scaled in place (not written where coef is 1). */
 typedef struct {
   void* param;
-  void* grad;
   void* exp_avg;    /* fp32, or e4m3 codes */
   void* exp_avg_sq; /* fp32, or e4m3 codes of its root */
   void* scales;     /* 8-bit moments: [ceil(numel / 256)][2] bytes */
@@ -395,16 +394,16 @@ typedef struct {
   int64_t numel;
 } unetk_adamw_tensor;
 int64_t unetk_grad_partials(int n_tensors);
-int64_t unetk_grad_sumsq(const unetk_adamw_tensor* tensors, int n_tensors, int dtype, double* partials, void* stream);
-int unetk_grad_clip(const unetk_adamw_tensor* tensors, int n_tensors, int dtype, const double* partials,
+int64_t unetk_grad_sumsq(void* const* grads, const int64_t* numel, int n_tensors, int dtype, double* partials, void* stream);
+int unetk_grad_clip(void* const* grads, const int64_t* numel, int n_tensors, int dtype, const double* partials,
                     int64_t n_partials, double max_norm, float* norm_out, void* stream);
-int64_t unetk_adamw_prepare(const unetk_adamw_tensor* tensors, int n_tensors, int dtype, double lr, const float* lr_dev,
-                            double beta1, double beta2, double weight_decay, int64_t seed, const float* found_inf,
+int64_t unetk_adamw_prepare(const unetk_adamw_tensor* tensors, void* const* grads, int n_tensors, int dtype, double lr,
+                            const float* lr_dev, double beta1, double beta2, double weight_decay, int64_t seed, const float* found_inf,
                             float* coefs, double* partials, void* stream);
-int unetk_adamw_update(const unetk_adamw_tensor* tensors, int n_tensors, int dtype, double beta1, double beta2,
+int unetk_adamw_update(const unetk_adamw_tensor* tensors, void* const* grads, int n_tensors, int dtype, double beta1, double beta2,
                        double eps, const float* grad_scale, const float* found_inf, const float* coefs,
                        const double* partials, int64_t n_partials, double max_norm, float* norm_out, void* stream);
-int unetk_adamw8_update(const unetk_adamw_tensor* tensors, int n_tensors, int dtype, double beta1, double beta2,
+int unetk_adamw8_update(const unetk_adamw_tensor* tensors, void* const* grads, int n_tensors, int dtype, double beta1, double beta2,
                         double eps, const float* grad_scale, const float* found_inf, const float* coefs,
                         const double* partials, int64_t n_partials, double max_norm, float* norm_out, void* stream);
 

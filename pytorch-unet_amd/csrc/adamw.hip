@@ -336,35 +336,51 @@ __global__ __launch_bounds__(256) void adamw8_update_kernel(Update8Table tb8, Be
 }
 
 // ---- host side
-// Fills the chunk map of tensors[0..n); false if they have more chunks than a launch can count.
-bool fill_chunks(const unetk_adamw_tensor* tensors, int n, Chunks* c) {
+// Fills the chunk map of n tensors; false if they have more chunks than a launch can count.
+template <typename Numel> bool fill_chunks(int n, Chunks* c, const Numel& numel) {
   int64_t total = 0;
   for (int i = 0; i < kTable; ++i) {
     c->first[i] = INT32_MAX;
-    c->numel[i] = 0;
     if (i >= n) continue;
-    c->numel[i] = tensors[i].numel;
+    c->numel[i] = numel(i);
     c->first[i] = (int)total;
-    total += (tensors[i].numel + kChunk - 1) / kChunk;
+    total += (c->numel[i] + kChunk - 1) / kChunk;
     if (total >= INT32_MAX) return false;
   }
   c->total = (int)total;
   return true;
 }
 
-int check_tensors(const unetk_adamw_tensor* tensors, int n, int dtype, bool params, bool steps, bool scales) {
-  if (!tensors || n <= 0) return UNETK_ERR_ARG;
+int check_grad(const void* grad, int64_t numel, uintptr_t mask) {
+  if (numel < 0) return UNETK_ERR_ARG;
+  if (numel == 0) return UNETK_OK;
+  if (numel >= (int64_t)(INT32_MAX - 1) * kChunk) return UNETK_ERR_SHAPE;
+  if (!grad) return UNETK_ERR_ARG;
+  return ((uintptr_t)grad & mask) ? UNETK_ERR_ALIGN : UNETK_OK;
+}
+
+int check_grads(void* const* grads, const int64_t* numel, int n, int dtype) {
+  if (!grads || !numel || n <= 0) return UNETK_ERR_ARG;
+  if (!unetk_dtype_ok(dtype)) return UNETK_ERR_DTYPE;
+  for (int i = 0; i < n; ++i)
+    if (const int rc = check_grad(grads[i], numel[i], unetk_esize(dtype) - 1)) return rc;
+  return UNETK_OK;
+}
+
+enum { kStep = 1, kMoments = 2, kScales = 4 };                       // what a call needs of a record
+int check_tensors(const unetk_adamw_tensor* tensors, void* const* grads, int n, int dtype, int need) {
+  if (!tensors || !grads || n <= 0) return UNETK_ERR_ARG;
   if (!unetk_dtype_ok(dtype)) return UNETK_ERR_DTYPE;
   const uintptr_t mask = unetk_esize(dtype) - 1;
   for (int i = 0; i < n; ++i) {
     const unetk_adamw_tensor& t = tensors[i];
-    if (t.numel < 0 || (steps && !t.step)) return UNETK_ERR_ARG;
-    if (steps && ((uintptr_t)t.step & 3)) return UNETK_ERR_ALIGN;
-    if (t.numel == 0) continue;
-    if (t.numel >= (int64_t)(INT32_MAX - 1) * kChunk) return UNETK_ERR_SHAPE;
-    if (!t.grad || (params && (!t.param || !t.exp_avg || !t.exp_avg_sq)) || (scales && !t.scales)) return UNETK_ERR_ARG;
-    if (((uintptr_t)t.grad & mask) || (params && ((uintptr_t)t.param & mask))) return UNETK_ERR_ALIGN;
-    if (params && !scales && (((uintptr_t)t.exp_avg | (uintptr_t)t.exp_avg_sq) & 3)) return UNETK_ERR_ALIGN;
+    if (const int rc = check_grad(grads[i], t.numel, mask)) return rc;
+    if ((need & kStep) && !t.step) return UNETK_ERR_ARG;
+    if ((need & kStep) && ((uintptr_t)t.step & 3)) return UNETK_ERR_ALIGN;
+    if (t.numel == 0 || !(need & kMoments)) continue;
+    if (!t.param || !t.exp_avg || !t.exp_avg_sq || ((need & kScales) && !t.scales)) return UNETK_ERR_ARG;
+    if ((uintptr_t)t.param & mask) return UNETK_ERR_ALIGN;
+    if (!(need & kScales) && (((uintptr_t)t.exp_avg | (uintptr_t)t.exp_avg_sq) & 3)) return UNETK_ERR_ALIGN;
   }
   return UNETK_OK;
 }
@@ -376,14 +392,16 @@ int check_clip(const double* partials, int64_t n_partials, double max_norm) {
 }
 
 inline int grid_of(int total, int most) { return total < 1 ? 1 : total < most ? total : most; }
+inline int table_of(int n_tensors, int at) { return n_tensors - at < kTable ? n_tensors - at : kTable; }
 
-template <typename Table> void fill_update(const unetk_adamw_tensor* tensors, int n, Table* u) {
+bool fill_update(const unetk_adamw_tensor* tensors, void* const* grads, int n, UpdateTable* u) {
   for (int i = 0; i < n; ++i) {
     u->param[i] = tensors[i].param;
-    u->grad[i] = tensors[i].grad;
+    u->grad[i] = grads[i];
     u->exp_avg[i] = tensors[i].exp_avg;
     u->exp_avg_sq[i] = tensors[i].exp_avg_sq;
   }
+  return fill_chunks(n, &u->c, [&](int i) { return tensors[i].numel; });
 }
 
 }  // namespace
@@ -395,111 +413,111 @@ int64_t unetk_grad_partials(int n_tensors) {
   return ((int64_t)n_tensors + kTable - 1) / kTable * kSumsqGrid;
 }
 
-int64_t unetk_grad_sumsq(const unetk_adamw_tensor* tensors, int n_tensors, int dtype, double* partials, void* stream) {
-  const int rc = check_tensors(tensors, n_tensors, dtype, false, false, false);
+int64_t unetk_grad_sumsq(void* const* grads, const int64_t* numel, int n_tensors, int dtype, double* partials, void* stream) {
+  const int rc = check_grads(grads, numel, n_tensors, dtype);
   if (rc != UNETK_OK) return rc;
   if (!partials) return UNETK_ERR_ARG;
   if ((uintptr_t)partials & 7) return UNETK_ERR_ALIGN;
   int64_t written = 0;
   for (int at = 0; at < n_tensors; at += kTable) {
-    const int n = n_tensors - at < kTable ? n_tensors - at : kTable;
-    GradTable tb = {};
-    if (!fill_chunks(tensors + at, n, &tb.c)) return UNETK_ERR_SHAPE;
-    for (int i = 0; i < n; ++i) tb.grad[i] = tensors[at + i].grad;
+    const int n = table_of(n_tensors, at);
+    GradTable tb;
+    if (!fill_chunks(n, &tb.c, [&](int i) { return numel[at + i]; })) return UNETK_ERR_SHAPE;
+    for (int i = 0; i < n; ++i) tb.grad[i] = grads[at + i];
     const int grid = grid_of(tb.c.total, kSumsqGrid);
-    UNETK_WITH_T(dtype, hipLaunchKernelGGL(grad_sumsq_kernel<T>, dim3(grid), dim3(256), 0, (hipStream_t)stream, tb, partials + written));
+    UNETK_WITH_T(dtype, hipLaunchKernelGGL(grad_sumsq_kernel<T>, dim3(grid), dim3(256), 0, (hipStream_t)stream, tb,
+                                           partials + written));
     UNETK_CHECK_LAUNCH();
     written += grid;
   }
   return written;
 }
 
-int unetk_grad_clip(const unetk_adamw_tensor* tensors, int n_tensors, int dtype, const double* partials,
+int unetk_grad_clip(void* const* grads, const int64_t* numel, int n_tensors, int dtype, const double* partials,
                     int64_t n_partials, double max_norm, float* norm_out, void* stream) {
-  int rc = check_tensors(tensors, n_tensors, dtype, false, false, false);
+  int rc = check_grads(grads, numel, n_tensors, dtype);
   if (rc == UNETK_OK) rc = check_clip(partials, n_partials, max_norm);
   if (rc != UNETK_OK) return rc;
   if (!partials) return UNETK_ERR_ARG;
   for (int at = 0; at < n_tensors; at += kTable) {
-    const int n = n_tensors - at < kTable ? n_tensors - at : kTable;
-    GradTable tb = {};
-    if (!fill_chunks(tensors + at, n, &tb.c)) return UNETK_ERR_SHAPE;
-    for (int i = 0; i < n; ++i) tb.grad[i] = tensors[at + i].grad;
+    const int n = table_of(n_tensors, at);
+    GradTable tb;
+    if (!fill_chunks(n, &tb.c, [&](int i) { return numel[at + i]; })) return UNETK_ERR_SHAPE;
+    for (int i = 0; i < n; ++i) tb.grad[i] = grads[at + i];
     const Clip clip{partials, (int)n_partials, (float)max_norm, nullptr, norm_out};
-    UNETK_WITH_T(dtype, hipLaunchKernelGGL(grad_clip_kernel<T>, dim3(grid_of(tb.c.total, kUpdateGrid)), dim3(256), 0, (hipStream_t)stream, tb, clip));
+    UNETK_WITH_T(dtype, hipLaunchKernelGGL(grad_clip_kernel<T>, dim3(grid_of(tb.c.total, kUpdateGrid)), dim3(256), 0,
+                                           (hipStream_t)stream, tb, clip));
     UNETK_CHECK_LAUNCH();
   }
   return UNETK_OK;
 }
 
-int64_t unetk_adamw_prepare(const unetk_adamw_tensor* tensors, int n_tensors, int dtype, double lr, const float* lr_dev,
-                            double beta1, double beta2, double weight_decay, int64_t seed, const float* found_inf, float* coefs,
-                            double* partials, void* stream) {
-  const int rc = check_tensors(tensors, n_tensors, dtype, false, true, false);
+int64_t unetk_adamw_prepare(const unetk_adamw_tensor* tensors, void* const* grads, int n_tensors, int dtype, double lr,
+                            const float* lr_dev, double beta1, double beta2, double weight_decay, int64_t seed,
+                            const float* found_inf, float* coefs, double* partials, void* stream) {
+  const int rc = check_tensors(tensors, grads, n_tensors, dtype, kStep);
   if (rc != UNETK_OK) return rc;
   if (!coefs) return UNETK_ERR_ARG;
   if (((uintptr_t)partials & 7) || ((uintptr_t)coefs & 15)) return UNETK_ERR_ALIGN;
   int64_t written = 0;
   for (int at = 0; at < n_tensors; at += kTable) {
-    const int n = n_tensors - at < kTable ? n_tensors - at : kTable;
-    PrepareTable tb = {};
-    if (!fill_chunks(tensors + at, n, &tb.c)) return UNETK_ERR_SHAPE;
-    for (int i = 0; i < n; ++i) tb.grad[i] = tensors[at + i].grad, tb.step[i] = tensors[at + i].step;
+    const int n = table_of(n_tensors, at);
+    PrepareTable tb;
+    if (!fill_chunks(n, &tb.c, [&](int i) { return tensors[at + i].numel; })) return UNETK_ERR_SHAPE;
+    for (int i = 0; i < n; ++i) tb.grad[i] = grads[at + i], tb.step[i] = tensors[at + i].step;
     Coefs* co = reinterpret_cast<Coefs*>(coefs) + at;
     if (partials) {
       const int grid = grid_of(tb.c.total, kSumsqGrid);
-      UNETK_WITH_T(dtype, hipLaunchKernelGGL((adamw_prepare_kernel<T, true>), dim3(grid), dim3(256), 0, (hipStream_t)stream, tb, n, lr,
-                                             lr_dev, beta1, beta2, weight_decay, (unsigned)seed, found_inf, co, partials + written));
+      UNETK_WITH_T(dtype, hipLaunchKernelGGL((adamw_prepare_kernel<T, true>), dim3(grid), dim3(256), 0, (hipStream_t)stream, tb, n,
+                                             lr, lr_dev, beta1, beta2, weight_decay, (unsigned)seed, found_inf, co,
+                                             partials + written));
       written += grid;
     } else {
-      hipLaunchKernelGGL((adamw_prepare_kernel<float, false>), dim3(1), dim3(256), 0, (hipStream_t)stream, tb, n, lr, lr_dev, beta1,
-                         beta2, weight_decay, (unsigned)seed, found_inf, co, (double*)nullptr);
+      hipLaunchKernelGGL((adamw_prepare_kernel<float, false>), dim3(1), dim3(256), 0, (hipStream_t)stream, tb, n, lr, lr_dev,
+                         beta1, beta2, weight_decay, (unsigned)seed, found_inf, co, (double*)nullptr);
     }
     UNETK_CHECK_LAUNCH();
   }
   return written;
 }
 
-int unetk_adamw_update(const unetk_adamw_tensor* tensors, int n_tensors, int dtype, double beta1, double beta2,
-                       double eps, const float* grad_scale, const float* found_inf, const float* coefs,
+int unetk_adamw_update(const unetk_adamw_tensor* tensors, void* const* grads, int n_tensors, int dtype, double beta1,
+                       double beta2, double eps, const float* grad_scale, const float* found_inf, const float* coefs,
                        const double* partials, int64_t n_partials, double max_norm, float* norm_out, void* stream) {
-  int rc = check_tensors(tensors, n_tensors, dtype, true, false, false);
+  int rc = check_tensors(tensors, grads, n_tensors, dtype, kMoments);
   if (rc == UNETK_OK) rc = check_clip(partials, n_partials, max_norm);
   if (rc != UNETK_OK) return rc;
   if (!coefs) return UNETK_ERR_ARG;
   const Betas b{(float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps};
   const Clip clip{partials, (int)n_partials, (float)max_norm, grad_scale, norm_out};
   for (int at = 0; at < n_tensors; at += kTable) {
-    const int n = n_tensors - at < kTable ? n_tensors - at : kTable;
-    UpdateTable tb = {};
-    if (!fill_chunks(tensors + at, n, &tb.c)) return UNETK_ERR_SHAPE;
-    fill_update(tensors + at, n, &tb);
+    UpdateTable tb;
+    if (!fill_update(tensors + at, grads + at, table_of(n_tensors, at), &tb)) return UNETK_ERR_SHAPE;
     const Coefs* co = reinterpret_cast<const Coefs*>(coefs) + at;
-    UNETK_WITH_T(dtype, hipLaunchKernelGGL(adamw_update_kernel<T>, dim3(grid_of(tb.c.total, kUpdateGrid)), dim3(256), 0, (hipStream_t)stream, tb, b,
-                                           co, found_inf, clip));
+    UNETK_WITH_T(dtype, hipLaunchKernelGGL(adamw_update_kernel<T>, dim3(grid_of(tb.c.total, kUpdateGrid)), dim3(256), 0,
+                                           (hipStream_t)stream, tb, b, co, found_inf, clip));
     UNETK_CHECK_LAUNCH();
   }
   return UNETK_OK;
 }
 
-int unetk_adamw8_update(const unetk_adamw_tensor* tensors, int n_tensors, int dtype, double beta1, double beta2,
-                        double eps, const float* grad_scale, const float* found_inf, const float* coefs,
+int unetk_adamw8_update(const unetk_adamw_tensor* tensors, void* const* grads, int n_tensors, int dtype, double beta1,
+                        double beta2, double eps, const float* grad_scale, const float* found_inf, const float* coefs,
                         const double* partials, int64_t n_partials, double max_norm, float* norm_out, void* stream) {
-  int rc = check_tensors(tensors, n_tensors, dtype, true, false, true);
+  int rc = check_tensors(tensors, grads, n_tensors, dtype, kMoments | kScales);
   if (rc == UNETK_OK) rc = check_clip(partials, n_partials, max_norm);
   if (rc != UNETK_OK) return rc;
   if (!coefs) return UNETK_ERR_ARG;
   const Betas b{(float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps};
   const Clip clip{partials, (int)n_partials, (float)max_norm, grad_scale, norm_out};
   for (int at = 0; at < n_tensors; at += kTable) {
-    const int n = n_tensors - at < kTable ? n_tensors - at : kTable;
-    Update8Table tb = {};
-    if (!fill_chunks(tensors + at, n, &tb.u.c)) return UNETK_ERR_SHAPE;
-    fill_update(tensors + at, n, &tb.u);
+    const int n = table_of(n_tensors, at);
+    Update8Table tb;
+    if (!fill_update(tensors + at, grads + at, n, &tb.u)) return UNETK_ERR_SHAPE;
     for (int i = 0; i < n; ++i) tb.scales[i] = tensors[at + i].scales;
     const Coefs* co = reinterpret_cast<const Coefs*>(coefs) + at;
-    UNETK_WITH_T(dtype, hipLaunchKernelGGL(adamw8_update_kernel<T>, dim3(grid_of(tb.u.c.total, kUpdateGrid)), dim3(256), 0, (hipStream_t)stream, tb, b,
-                                           co, found_inf, clip));
+    UNETK_WITH_T(dtype, hipLaunchKernelGGL(adamw8_update_kernel<T>, dim3(grid_of(tb.u.c.total, kUpdateGrid)), dim3(256), 0,
+                                           (hipStream_t)stream, tb, b, co, found_inf, clip));
     UNETK_CHECK_LAUNCH();
   }
   return UNETK_OK;

@@ -12,7 +12,9 @@ buffer of unetk.ddp.FlatGrads, the optimizer state is two more flat buffers, and
 (or the flat buffers above), decoupled weight decay, moments in 32 or in 8 bits, the clip in front of the step or by itself.
 """
 import contextlib
-import ctypes
+from array import array
+from itertools import chain
+from operator import is_
 
 import torch
 
@@ -141,9 +143,20 @@ class ClipRMSprop(torch.optim.Optimizer):
 
 
 # ---------------------------------------------------------------------------------------- many tensors at once
-_WORDS = 7                      # unetk_adamw_tensor: param, grad, exp_avg, exp_avg_sq, scales, step, numel
 BLOCK = 256                     # elements that share one scale per moment (unetk_adamw8_update)
 _CODE, _SCALE = torch.float8_e4m3fn, torch.float8_e8m0fnu
+
+
+_TYPES = {torch.float32, torch.bfloat16, torch.float16}
+
+# one C call per tensor each: a step of small tensors is bound by what the host asks of them
+_get_pointer, _get_numel, _get_device = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device
+_get_contiguous, _get_dtype, _get_stride = torch.Tensor.is_contiguous, torch.Tensor.dtype.__get__, torch.Tensor.stride
+_get_wanted = torch.Tensor.requires_grad.__get__
+
+
+def _address(words):
+    return words.buffer_info()[0]
 
 
 def _on_device(device):
@@ -191,38 +204,34 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError(f'clip_grad_norm_: max_norm must not be negative, got {max_norm}')
-    grads = [p.grad for p in parameters if p.grad is not None]
+    grads = [g for g in [p.grad for p in parameters] if g is not None]
     if not grads:
         return torch.tensor(0.0)
-    device = grads[0].device
-    by_type = {}
-    for g in grads:
-        _require(g, 'gradients', 'clip_grad_norm_')
-        if g.device != device:
-            raise RuntimeError('clip_grad_norm_: gradients must be on one device')
-        by_type.setdefault(g.dtype, []).append(g)
-    if len({id(g) for g in grads}) != len(grads):
+    if len(set(map(id, grads))) != len(grads):
         raise ValueError('clip_grad_norm_: a parameter appears twice')
+    if len(set(map(_get_device, grads))) != 1:
+        raise RuntimeError('clip_grad_norm_: gradients must be on one device')
+    types = set(map(_get_dtype, grads))
+    if not grads[0].is_cuda or not types <= _TYPES or not all(map(_get_contiguous, grads)):
+        for g in grads:
+            _require(g, 'gradients', 'clip_grad_norm_')
+    sets = [(dtype_code(t), grads if len(types) == 1 else [g for g in grads if g.dtype == t]) for t in types]
+    device = grads[0].device
     with _on_device(device):
         stream = stream_ptr()
-        tables = []
-        for dtype, gs in by_type.items():
-            t = (ctypes.c_int64 * (_WORDS * len(gs)))()
-            t[1::_WORDS] = [g.data_ptr() for g in gs]
-            t[6::_WORDS] = [g.numel() for g in gs]
-            tables.append((t, len(gs), dtype_code(dtype)))
-        partials = torch.empty(sum(fn['unetk_grad_partials'](n) for _, n, _ in tables), dtype=torch.float64, device=device)
+        sets = [(code, len(gs), array('q', map(_get_pointer, gs)), array('q', map(_get_numel, gs))) for code, gs in sets]
+        partials = torch.empty(sum(fn['unetk_grad_partials'](n) for _, n, _, _ in sets), dtype=torch.float64, device=device)
         norm = torch.empty((), dtype=torch.float32, device=device)
-        count = 0
-        for t, n, code in tables:
-            count += _written(fn['unetk_grad_sumsq'](ctypes.addressof(t), n, code, partials.data_ptr() + 8 * count, stream),
+        at, count = partials.data_ptr(), 0
+        for code, n, pointers, numel in sets:
+            count += _written(fn['unetk_grad_sumsq'](_address(pointers), _address(numel), n, code, at + 8 * count, stream),
                               'unetk_grad_sumsq')
         if error_if_nonfinite:
             total = partials[:count].sum().sqrt()
             if not bool(torch.isfinite(total)):
                 raise RuntimeError('clip_grad_norm_: the norm of the gradients is not finite, so they cannot be clipped')
-        for t, n, code in tables:
-            check(fn['unetk_grad_clip'](ctypes.addressof(t), n, code, partials.data_ptr(), count, max_norm, norm.data_ptr(),
+        for code, n, pointers, numel in sets:
+            check(fn['unetk_grad_clip'](_address(pointers), _address(numel), n, code, at, count, max_norm, norm.data_ptr(),
                                         stream), 'unetk_grad_clip')
     torch.autograd.graph.increment_version(grads)
     return norm
@@ -288,6 +297,7 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f'AdamW: state_bits must be 8 or 32, got {state_bits}')
         self.state_bits, self.min_8bit_numel, self.seed = state_bits, int(min_8bit_numel), int(seed) & 0xFFFFFFFF
         self.total_norm = None
+        self._plan = None
         if self.fg is not None:          # net.parameters() order, as a stock optimizer numbers its state
             params = [p for p in self.fg.module_order if id(p) in self.fg.offsets]
             for p in params:             # laid out like its view of the flat gradients
@@ -296,6 +306,7 @@ class AdamW(torch.optim.Optimizer):
 
     def add_param_group(self, group):
         super().add_param_group(group)
+        self._plan = None
         try:
             self._check_group(self.param_groups[-1])
         except Exception:
@@ -380,14 +391,11 @@ class AdamW(torch.optim.Optimizer):
             for k in ('lr', 'betas', 'eps', 'weight_decay', 'max_norm', 'initial_lr'):
                 if k in g:
                     own[k] = g[k]
+        self._plan = None
         self.state.clear()
         self.state.update(state)
 
     # ---- step
-    def _gradient(self, p):
-        return p.grad if self.fg is None else self.fg.views.get(p)
-
-    @torch.no_grad()
     def step(self, closure=None):
         loss = None
         if closure is not None:
@@ -395,85 +403,140 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         if self.fg is not None and self.fg.flat is None:
             raise RuntimeError('AdamW.step: no gradients (run backward through the UNet first)')
-        jobs, stepped = self._jobs()
-        if stepped:
-            with _on_device(stepped[0].device):
-                self._launch(jobs, stepped[0].device)
+        plan = self._plan
+        pointers = plan.pointers(self) if plan is not None else None
+        if pointers is None:                             # the first step, or something moved, came or went
+            plan = self._plan = None
+            with torch.no_grad():
+                plan, pointers, copies = self._make_plan()
+        if plan.params:
+            with _on_device(plan.device):
+                self._launch(plan, pointers)
             # the kernels wrote the parameters behind PyTorch's back: bump their version counters like any in-place op
-            torch.autograd.graph.increment_version(stepped)
+            torch.autograd.graph.increment_version(plan.params)
+        self._plan = plan
         if self.fg is not None:
             self.fg.consume()
         return loss
 
-    def _jobs(self):
-        """[(group, type, bits, number of tensors, table, gradients)] and the parameters that take part."""
-        jobs, stepped = [], []
-        for group in self.param_groups:
-            rows = {}
+    def _make_plan(self):
+        """Looks every tensor over: the plan of this step, the gradients' pointers, and copies of gradients that lie unlike their
+        parameters (to be kept until the launch)."""
+        sets, absent, copies = {}, [], []
+        for at, group in enumerate(self.param_groups):
             for p in group['params']:
-                g = self._gradient(p)
+                # the flat buffer has room for frozen parameters too
+                g = p.grad if self.fg is None else self.fg.views.get(p) if p.requires_grad else None
                 if g is None:
+                    absent.append(p)
                     continue
-                st = self.state.get(p)
-                if not st:
-                    st = self.state[p] = self._new_state(p)
                 if self.fg is not None and not p.is_contiguous():
                     p.data = p.data.contiguous()
                 _require(p, 'parameters')
+                st = self.state.get(p)
+                if not st:
+                    st = self.state[p] = self._new_state(p)
                 bits = self._check_state(p, st)
                 if g.layout != torch.strided or g.dtype != p.dtype or g.device != p.device or g.shape != p.shape:
-                    raise RuntimeError(f'AdamW: a gradient must be a strided tensor of its parameter\'s type, shape and device')
+                    raise RuntimeError("AdamW: a gradient must be a strided tensor of its parameter's type, shape and device")
                 if g.stride() != p.stride():
                     g = torch.empty_like(p).copy_(g)
-                second = st['exp_avg_root' if bits == 8 else 'exp_avg_sq']
-                rows.setdefault((p.dtype, bits), []).append(
-                    (g, (p.data_ptr(), g.data_ptr(), st['exp_avg'].data_ptr(), second.data_ptr(),
-                         st['scales'].data_ptr() if bits == 8 else 0, st['step'].data_ptr(), p.numel())))
-                stepped.append(p)
-            for (dtype, bits), rs in rows.items():
-                table = (ctypes.c_int64 * (_WORDS * len(rs)))(*[w for _, r in rs for w in r])
-                jobs.append((group, dtype_code(dtype), bits, len(rs), table, [g for g, _ in rs]))
-        return jobs, stepped
+                    copies.append(g)
+                sets.setdefault((at, p.dtype, bits), []).append((p, st, g))
+        plan = _Plan(self, sets, absent)
+        return plan, array('q', [g.data_ptr() for rows in sets.values() for _, _, g in rows]), copies
 
-    def _launch(self, jobs, device):
-        stream = stream_ptr()
+    def _launch(self, plan, pointers):
+        stream, device = stream_ptr(), plan.device
         max_norm = self.param_groups[0]['max_norm']
         grad_scale, found_inf = getattr(self, 'grad_scale', None), getattr(self, 'found_inf', None)
         for t in (grad_scale, found_inf):
             if t is not None and (t.dtype != torch.float32 or t.device != device or t.numel() != 1):
-                raise RuntimeError('AdamW: grad_scale and found_inf must be fp32 scalars on the parameters\' device')
+                raise RuntimeError("AdamW: grad_scale and found_inf must be fp32 scalars on the parameters' device")
         scale_ptr = grad_scale.data_ptr() if grad_scale is not None else None
         found_ptr = found_inf.data_ptr() if found_inf is not None else None
         # scratch of this call alone, from the allocator of the stream it runs on: calls share none of it
-        sizes = [int(fn['unetk_grad_partials'](n)) if max_norm is not None else 0 for _, _, _, n, _, _ in jobs]
-        tensors = sum(job[3] for job in jobs)
-        scratch = torch.empty(2 * tensors + sum(sizes), dtype=torch.float64, device=device)
-        coefs = scratch.data_ptr()
-        partials = coefs + 16 * tensors if max_norm is not None else None
+        scratch = torch.empty(plan.words[max_norm is not None], dtype=torch.float64, device=device)
+        coefs, partials, norm_ptr, count = scratch.data_ptr(), None, None, 0
         if max_norm is not None:
             self.total_norm = torch.empty((), dtype=torch.float32, device=device)
-        norm_ptr = self.total_norm.data_ptr() if max_norm is not None else None
-        count, at = 0, coefs
-        for group, code, bits, n, table, _ in jobs:
+            partials, norm_ptr = coefs + 16 * len(plan.params), self.total_norm.data_ptr()
+        grads = _address(pointers)
+        for at, code, bits, first, n, table in plan.sets:
+            group = self.param_groups[at]
             lr, lr_ptr = group['lr'], None
             if isinstance(lr, torch.Tensor):
                 if lr.is_cuda:
                     if lr.dtype != torch.float32 or lr.device != device or lr.numel() != 1:
-                        raise RuntimeError('AdamW: a tensor lr must be an fp32 scalar on the parameters\' device')
+                        raise RuntimeError("AdamW: a tensor lr must be an fp32 scalar on the parameters' device")
                     lr, lr_ptr = 0.0, lr.data_ptr()
                 else:
                     lr = float(lr)
-            count += _written(fn['unetk_adamw_prepare'](ctypes.addressof(table), n, code, float(lr), lr_ptr, *group['betas'],
-                                                        group['weight_decay'], self.seed, found_ptr, at,
+            count += _written(fn['unetk_adamw_prepare'](table, grads + 8 * first, n, code, lr, lr_ptr, *group['betas'],
+                                                        group['weight_decay'], self.seed, found_ptr, coefs + 16 * first,
                                                         partials + 8 * count if partials else None, stream),
                               'unetk_adamw_prepare')
-            at += 16 * n
-        at = coefs
-        for group, code, bits, n, table, _ in jobs:
-            name = 'unetk_adamw_update' if bits == 32 else 'unetk_adamw8_update'
-            check(fn[name](ctypes.addressof(table), n, code, *group['betas'], group['eps'], scale_ptr, found_ptr, at, partials,
-                           count, max_norm or 0.0, norm_ptr, stream), name)
-            at += 16 * n
+        for at, code, bits, first, n, table in plan.sets:
+            group, name = self.param_groups[at], 'unetk_adamw_update' if bits == 32 else 'unetk_adamw8_update'
+            check(fn[name](table, grads + 8 * first, n, code, *group['betas'], group['eps'], scale_ptr, found_ptr,
+                           coefs + 16 * first, partials, count, max_norm or 0.0, norm_ptr, stream), name)
+
+
+class _Plan:
+    """What one step found out about its tensors, for the next one: everything but the gradients' pointers, and how to tell that
+    it still holds.  It keeps the tensors it speaks of alive, so an address in it cannot become another tensor's."""
+
+    def __init__(self, opt, sets, absent):
+        rows = [r for rs in sets.values() for r in rs]
+        self.params, self.absent = [p for p, _, _ in rows], absent
+        self.device = rows[0][0].device if rows else None
+        self.counts = [len(g['params']) for g in opt.param_groups]
+        self.sets, self.tables, first = [], [], 0
+        for (at, dtype, bits), rs in sets.items():
+            second = 'exp_avg_root' if bits == 8 else 'exp_avg_sq'
+            table = array('q', [w for p, st, _ in rs for w in
+                                (p.data_ptr(), st['exp_avg'].data_ptr(), st[second].data_ptr(),
+                                 st['scales'].data_ptr() if bits == 8 else 0, st['step'].data_ptr(), p.numel())])
+            self.tables.append(table)
+            self.sets.append((at, dtype_code(dtype), bits, first, len(rs), _address(table)))
+            first += len(rs)
+        self.words = [2 * first, 2 * first + sum(int(fn['unetk_grad_partials'](s[4])) for s in self.sets)]
+        self.state = list(opt.state.values())
+        self.kept = list(chain.from_iterable(map(dict.values, self.state)))
+        self.where = list(map(_get_pointer, self.params)) + list(map(_get_pointer, self.kept))
+        self.types, self.numel = list(map(_get_dtype, self.params)), list(map(_get_numel, self.params))
+        self.contiguous = all(map(_get_contiguous, self.params))
+        self.strides = None if self.contiguous else list(map(_get_stride, self.params))
+        if opt.fg is not None:
+            self.offsets = [4 * opt.fg.offsets[id(p)] for p in self.params]
+
+    def pointers(self, opt):
+        """The gradients' pointers if the plan holds for this step, else None."""
+        params = self.params
+        now = list(opt.state.values())
+        if [len(g['params']) for g in opt.param_groups] != self.counts or len(now) != len(self.state) or \
+                not all(map(is_, now, self.state)):
+            return None
+        if list(map(_get_pointer, params)) + list(map(_get_pointer, chain.from_iterable(map(dict.values, now)))) != self.where:
+            return None
+        if not all(map(_get_contiguous, params)) if self.contiguous else list(map(_get_stride, params)) != self.strides:
+            return None
+        if opt.fg is not None:
+            if not all(map(_get_wanted, params)) or any(map(_get_wanted, self.absent)):
+                return None
+            base = opt.fg.flat.data_ptr()
+            return array('q', [base + o for o in self.offsets])
+        grads = [p.grad for p in params]
+        if any(p.grad is not None for p in self.absent):
+            return None
+        try:
+            if list(map(_get_dtype, grads)) != self.types or list(map(_get_numel, grads)) != self.numel:
+                return None
+            if not all(map(_get_contiguous, grads)) if self.contiguous else list(map(_get_stride, grads)) != self.strides:
+                return None
+            return array('q', map(_get_pointer, grads))
+        except (TypeError, RuntimeError):                # a gradient that is None, or not a strided tensor
+            return None
 
 
 def _fit_moments(p, st, bits):

@@ -20,49 +20,51 @@ def optim():
     return optim
 
 
-def table(*rows):
-    return (ctypes.c_int64 * (7 * len(rows)))(*[w for r in rows for w in r])
+def words(*values):
+    return (ctypes.c_int64 * len(values))(*values)
 
 
-ROW = (64, 64, 64, 64, 64, 64, 10)
+ROW = (64, 64, 64, 64, 64, 10)                      # param, exp_avg, exp_avg_sq, scales, step, numel
 
 
 def test_entry_points_refuse_before_launch(nat):
-    fn = nat.fn
-    good, a = table(ROW), ctypes.addressof
+    fn, a = nat.fn, ctypes.addressof
+    good, grad = words(*ROW), words(64)
 
-    def prepare(t, n=1, dtype=nat.F32, coefs=64, partials=None):
-        return fn['unetk_adamw_prepare'](a(t) if t else None, n, dtype, 1e-3, None, 0.9, 0.999, 0.0, 0, None, coefs, partials, None)
+    def prepare(t=good, g=grad, n=1, dtype=nat.F32, coefs=64, partials=None):
+        return fn['unetk_adamw_prepare'](a(t) if t else None, a(g) if g else None, n, dtype, 1e-3, None, 0.9, 0.999, 0.0, 0, None,
+                                         coefs, partials, None)
 
-    def update(name, t, n=1, dtype=nat.F32, coefs=64, partials=None, count=0, max_norm=1.0):
-        return fn[name](a(t) if t else None, n, dtype, 0.9, 0.999, 1e-8, None, None, coefs, partials, count, max_norm, None, None)
+    def update(name, t=good, g=grad, n=1, dtype=nat.F32, coefs=64, partials=None, count=0, max_norm=1.0):
+        return fn[name](a(t) if t else None, a(g) if g else None, n, dtype, 0.9, 0.999, 1e-8, None, None, coefs, partials, count,
+                        max_norm, None, None)
 
-    assert prepare(None) == -5 and prepare(good, 0) == -5 and prepare(good, dtype=9) == -2 and prepare(good, coefs=None) == -5
-    assert prepare(good, coefs=72) == -3 and prepare(good, partials=12) == -3
-    assert prepare(table(ROW[:5] + (0, 10))) == -5 and prepare(table(ROW[:5] + (66, 10))) == -3      # step
-    assert prepare(table(ROW[:6] + (-1,))) == -5 and prepare(table(ROW[:6] + (1 << 60,))) == -1      # numel
+    assert prepare(None) == -5 and prepare(g=None) == -5 and prepare(n=0) == -5 and prepare(dtype=9) == -2
+    assert prepare(coefs=None) == -5 and prepare(coefs=72) == -3 and prepare(partials=12) == -3
+    assert prepare(words(*ROW[:4], 0, 10)) == -5 and prepare(words(*ROW[:4], 66, 10)) == -3            # step
+    assert prepare(words(*ROW[:5], -1)) == -5 and prepare(words(*ROW[:5], 1 << 60)) == -1              # numel
+    assert prepare(g=words(0)) == -5 and prepare(g=words(66)) == -3
     for name in ('unetk_adamw_update', 'unetk_adamw8_update'):
-        assert update(name, None) == -5 and update(name, good, -1) == -5 and update(name, good, dtype=3) == -2
-        assert update(name, good, coefs=None) == -5
-        assert update(name, good, partials=64, count=0) == -5 and update(name, good, partials=None, count=4) == -5
-        assert update(name, good, partials=12, count=4) == -3
+        assert update(name, None) == -5 and update(name, g=None) == -5 and update(name, n=-1) == -5 and update(name, dtype=3) == -2
+        assert update(name, coefs=None) == -5
+        assert update(name, partials=64, count=0) == -5 and update(name, partials=None, count=4) == -5
+        assert update(name, partials=12, count=4) == -3
         for bad in (-1.0, float('nan')):
-            assert update(name, good, partials=64, count=4, max_norm=bad) == -5
-        for k in range(4):
+            assert update(name, partials=64, count=4, max_norm=bad) == -5
+        for k in range(3):
             r = list(ROW)
             r[k] = 0
-            assert update(name, table(r)) == -5
-        r = list(ROW)
-        r[0] = 66                                                       # an fp32 parameter at two bytes
-        assert update(name, table(ROW, r), 2) == -3
-    r = list(ROW)
-    r[4] = 0
-    assert update('unetk_adamw8_update', table(r)) == -5
+            assert update(name, words(*r)) == -5
+        assert update(name, g=words(0)) == -5
+        assert update(name, words(*ROW, 66, *ROW[1:]), words(64, 64), 2) == -3                         # an fp32 parameter at two bytes
+    assert update('unetk_adamw8_update', words(*ROW[:3], 0, *ROW[4:])) == -5
     assert fn['unetk_grad_partials'](0) == -5 and fn['unetk_grad_partials'](65) == 2 * fn['unetk_grad_partials'](64)
-    assert fn['unetk_grad_sumsq'](a(good), 1, nat.F32, None, None) == -5
-    assert fn['unetk_grad_sumsq'](a(good), 1, nat.F32, 12, None) == -3
-    assert fn['unetk_grad_clip'](a(good), 1, nat.F32, None, 0, 1.0, None, None) == -5
-    assert fn['unetk_grad_clip'](a(good), 1, nat.BF16, 64, 3, float('nan'), None, None) == -5
+    ten = words(10)
+    assert fn['unetk_grad_sumsq'](a(grad), a(ten), 1, nat.F32, None, None) == -5
+    assert fn['unetk_grad_sumsq'](a(grad), a(ten), 1, nat.F32, 12, None) == -3
+    assert fn['unetk_grad_sumsq'](a(grad), None, 1, nat.F32, 64, None) == -5
+    assert fn['unetk_grad_clip'](a(grad), a(ten), 1, nat.F32, None, 0, 1.0, None, None) == -5
+    assert fn['unetk_grad_clip'](a(grad), a(ten), 1, nat.BF16, 64, 3, float('nan'), None, None) == -5
 
 
 def test_no_cpu_fallback_and_bad_arguments(optim):

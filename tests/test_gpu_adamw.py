@@ -595,3 +595,83 @@ def test_the_trainer_in_mixed_precision_with_8bit_moments(optim, amp_dtype):
                    1.0, 0, tr.optimizer.total_norm)
     kinds = {'scales' in tr.optimizer.state[p] for p in net.parameters()}
     assert kinds == {True, False}
+
+
+# ------------------------------------------------------------------------------- what is carried from step to step
+@pytest.mark.parametrize('bits', [32, 8])
+def test_whatever_moves_between_steps_is_noticed(optim, bits):
+    """The checks of one step serve the next; everything that may change in between has to end that.  The twin forgets them
+    before each step."""
+    sizes = [5000, 12, 4097, 300]
+    params, twin = make(sizes, torch.float32), make(sizes, torch.float32)
+    kw = dict(HYPER, max_norm=0.3, state_bits=bits)
+    opt, ref = optim.AdamW(params, **kw), optim.AdamW(twin, **kw)
+    g = torch.Generator().manual_seed(6)
+    hold = []
+
+    def new_data(o, ps):
+        hold.append(ps[0].data)
+        ps[0].data = ps[0].data.clone() * 0.5
+
+    def new_entry(o, ps):
+        hold.append(o.state[ps[2]]['exp_avg'])
+        x = o.state[ps[2]]['exp_avg']
+        o.state[ps[2]]['exp_avg'] = torch.zeros_like(x) if bits == 32 else torch.zeros_like(x, dtype=torch.uint8).view(x.dtype)
+
+    def moved_entry(o, ps):
+        o.state[ps[1]]['exp_avg_sq'].data = o.state[ps[1]]['exp_avg_sq'].data.clone()
+        o.state[ps[1]]['exp_avg_sq'].mul_(2.0)
+
+    def new_state(o, ps):
+        o.state[ps[3]] = {k: v.clone() for k, v in o.state[ps[3]].items()}
+        o.state[ps[3]]['step'].fill_(7.0)
+
+    def no_state(o, ps):
+        hold.append(o.state.pop(ps[1]))
+
+    def no_gradient(o, ps):
+        ps[2].grad = None
+
+    def strided_gradient(o, ps):
+        ps[0].grad = torch.stack([ps[0].grad, -ps[0].grad], 1)[:, 0]
+
+    def new_group(o, ps):
+        ps.append(make([4500], torch.float32, seed=12)[0])
+        o.add_param_group({'params': [ps[-1]], 'lr': 0.5, 'betas': (0.5, 0.6)})
+
+    def new_rate(o, ps):
+        o.param_groups[0]['lr'] *= 3
+        o.param_groups[0]['betas'] = (0.5, 0.9)
+
+    for change in (None, new_data, None, new_entry, moved_entry, new_state, no_state, no_gradient, None, strided_gradient, new_group,
+                   new_rate, None):
+        for i in range(len(params)):
+            new = torch.randn(params[i].numel(), generator=g).cuda()
+            params[i].grad, twin[i].grad = new, new.clone()
+        if change is not None:
+            change(opt, params), change(ref, twin)
+        ref._plan = None
+        opt.step(), ref.step()
+        assert all(torch.equal(p, q) for p, q in zip(params, twin)), change
+        assert [float(opt.state[p]['step']) for p in params] == [float(ref.state[q]['step']) for q in twin], change
+    assert float(opt.state[params[3]]['step']) == 15.0 and float(opt.state[params[2]]['step']) == 12.0
+
+
+def test_frozen_parameters_of_a_flat_buffer_stay(optim):
+    from unet import UNet
+    from unetk.ddp import FlatGrads
+    torch.manual_seed(0)
+    net = UNet(3, 2, False).cuda()
+    fg = FlatGrads(net, grads_to_autograd=False)
+    opt = optim.AdamW(fg, lr=1e-2, weight_decay=0.5)
+    with pytest.raises(RuntimeError, match='no gradients'):
+        opt.step()
+    frozen = net.inc.double_conv[0].weight
+    for k in range(4):
+        frozen.requires_grad_(k == 2)
+        fg.initial_grads()
+        fg.flat.normal_()
+        before = frozen.detach().clone(), net.outc.conv.weight.detach().clone()
+        opt.step()
+        assert torch.equal(frozen, before[0]) == (k != 2) and not torch.equal(net.outc.conv.weight, before[1])
+    assert float(opt.state[frozen]['step']) == 1.0 and float(opt.state[net.outc.conv.weight]['step']) == 4.0
