@@ -364,7 +364,7 @@ int unetk_clip_rmsprop_step(float* param, float* grad, float* square_avg, float*
  * The gradient is left as it is.  Moments and all arithmetic are fp32 (the partial sums and bias corrections fp64);
  * a parameter of 16 bits is rounded once, to nearest.
  *
- * Moments in 8 bits (unetk_adamw8_update): a block is 256 consecutive elements of a tensor, the last one shorter.
+ * Moments in 8 bits (records whose `scales` is not NULL): a block is 256 consecutive elements of a tensor, the last one shorter.
  * exp_avg holds m and exp_avg_sq holds the ROOT r = sqrt(v) as fp8 e4m3 codes of value / 2^k; `scales` holds 127 + k in a byte,
  * [blocks][2]: m's and r's.  k is the smallest integer >= -127 with |value| <= 448 * 2^k for the block's finite values.
  * Codes are rounded stochastically, |code| = floor(|x| / ulp + (u + 1/2) / 65536) * ulp with ulp the e4m3 spacing at
@@ -379,7 +379,7 @@ int unetk_clip_rmsprop_step(float* param, float* grad, float* square_avg, float*
  * unetk_adamw_prepare: adds 1 to every `step`, writes each tensor's bias corrections to `coefs` (16 bytes a tensor) and, if
  *   `partials` is not NULL, sums of squares of the gradients to `partials`.  Returns how many of them it wrote (at most
  *   unetk_grad_partials(n_tensors)) or a negative error.  lr_dev (may be NULL): lr is read from there.
- * unetk_adamw_update / unetk_adamw8_update: the update; `partials`, `n_partials`: those of ALL sets that the norm covers
+ * unetk_adamw_update: the update; `partials`, `n_partials`: those of ALL sets that the norm covers
  *   (NULL and 0 without a clip).  norm_out (may be NULL) receives the norm.
  * grad_scale, found_inf (device, may be NULL): torch.amp.GradScaler's; found_inf != 0 skips the step, its count included.
  *
@@ -389,7 +389,7 @@ typedef struct {
   void* param;
   void* exp_avg;    /* fp32, or e4m3 codes */
   void* exp_avg_sq; /* fp32, or e4m3 codes of its root */
-  void* scales;     /* 8-bit moments: [ceil(numel / 256)][2] bytes */
+  void* scales;     /* 8-bit moments: [ceil(numel / 256)][2] bytes; NULL: the moments are fp32 */
   float* step;
   int64_t numel;
 } unetk_adamw_tensor;
@@ -403,9 +403,6 @@ int64_t unetk_adamw_prepare(const unetk_adamw_tensor* tensors, void* const* grad
 int unetk_adamw_update(const unetk_adamw_tensor* tensors, void* const* grads, int n_tensors, int dtype, double beta1, double beta2,
                        double eps, const float* grad_scale, const float* found_inf, const float* coefs,
                        const double* partials, int64_t n_partials, double max_norm, float* norm_out, void* stream);
-int unetk_adamw8_update(const unetk_adamw_tensor* tensors, void* const* grads, int n_tensors, int dtype, double beta1, double beta2,
-                        double eps, const float* grad_scale, const float* found_inf, const float* coefs,
-                        const double* partials, int64_t n_partials, double max_norm, float* norm_out, void* stream);
 
 /* ---- input formatting: BasicDataset.preprocess, utils/data_loading.py:65-91 ----------
  * The reference resizes on the CPU with Pillow (`pil_img.resize`, :69: BICUBIC for images, NEAREST for masks) and

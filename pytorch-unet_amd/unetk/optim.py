@@ -143,7 +143,7 @@ class ClipRMSprop(torch.optim.Optimizer):
 
 
 # ---------------------------------------------------------------------------------------- many tensors at once
-BLOCK = 256                     # elements that share one scale per moment (unetk_adamw8_update)
+BLOCK = 256                     # elements that share one scale per moment (unetk_adamw_update)
 _CODE, _SCALE = torch.float8_e4m3fn, torch.float8_e8m0fnu
 
 
@@ -267,7 +267,7 @@ def quantize_moment(x, keep_positive=False):
 
 class AdamW(torch.optim.Optimizer):
     """AdamW over any list of parameters, the whole step in two launches per 64 tensors of one type (include/unetk.h:
-    unetk_adamw_prepare, unetk_adamw_update, unetk_adamw8_update), with clip_grad_norm_(max_norm) over all of them in front.
+    unetk_adamw_prepare, unetk_adamw_update), with clip_grad_norm_(max_norm) over all of them in front.
 
     params: an iterable of tensors or of parameter groups, on one GPU, in fp32, bf16 or fp16; or a unetk.ddp.FlatGrads, whose
     flat gradient buffer is then read in place.  Any dense memory layout; a gradient that is laid out unlike its parameter is
@@ -436,13 +436,13 @@ class AdamW(torch.optim.Optimizer):
                 st = self.state.get(p)
                 if not st:
                     st = self.state[p] = self._new_state(p)
-                bits = self._check_state(p, st)
+                self._check_state(p, st)
                 if g.layout != torch.strided or g.dtype != p.dtype or g.device != p.device or g.shape != p.shape:
                     raise RuntimeError("AdamW: a gradient must be a strided tensor of its parameter's type, shape and device")
                 if g.stride() != p.stride():
                     g = torch.empty_like(p).copy_(g)
                     copies.append(g)
-                sets.setdefault((at, p.dtype, bits), []).append((p, st, g))
+                sets.setdefault((at, p.dtype), []).append((p, st, g))
         plan = _Plan(self, sets, absent)
         return plan, array('q', [g.data_ptr() for rows in sets.values() for _, _, g in rows]), copies
 
@@ -462,7 +462,7 @@ class AdamW(torch.optim.Optimizer):
             self.total_norm = torch.empty((), dtype=torch.float32, device=device)
             partials, norm_ptr = coefs + 16 * len(plan.params), self.total_norm.data_ptr()
         grads = _address(pointers)
-        for at, code, bits, first, n, table in plan.sets:
+        for at, code, first, n, table in plan.sets:
             group = self.param_groups[at]
             lr, lr_ptr = group['lr'], None
             if isinstance(lr, torch.Tensor):
@@ -476,10 +476,11 @@ class AdamW(torch.optim.Optimizer):
                                                         group['weight_decay'], self.seed, found_ptr, coefs + 16 * first,
                                                         partials + 8 * count if partials else None, stream),
                               'unetk_adamw_prepare')
-        for at, code, bits, first, n, table in plan.sets:
-            group, name = self.param_groups[at], 'unetk_adamw_update' if bits == 32 else 'unetk_adamw8_update'
-            check(fn[name](table, grads + 8 * first, n, code, *group['betas'], group['eps'], scale_ptr, found_ptr,
-                           coefs + 16 * first, partials, count, max_norm or 0.0, norm_ptr, stream), name)
+        for at, code, first, n, table in plan.sets:
+            group = self.param_groups[at]
+            check(fn['unetk_adamw_update'](table, grads + 8 * first, n, code, *group['betas'], group['eps'], scale_ptr, found_ptr,
+                                           coefs + 16 * first, partials, count, max_norm or 0.0, norm_ptr, stream),
+                  'unetk_adamw_update')
 
 
 class _Plan:
@@ -492,15 +493,15 @@ class _Plan:
         self.device = rows[0][0].device if rows else None
         self.counts = [len(g['params']) for g in opt.param_groups]
         self.sets, self.tables, first = [], [], 0
-        for (at, dtype, bits), rs in sets.items():
-            second = 'exp_avg_root' if bits == 8 else 'exp_avg_sq'
+        for (at, dtype), rs in sets.items():
             table = array('q', [w for p, st, _ in rs for w in
-                                (p.data_ptr(), st['exp_avg'].data_ptr(), st[second].data_ptr(),
-                                 st['scales'].data_ptr() if bits == 8 else 0, st['step'].data_ptr(), p.numel())])
+                                (p.data_ptr(), st['exp_avg'].data_ptr(),
+                                 st['exp_avg_root' if 'scales' in st else 'exp_avg_sq'].data_ptr(),
+                                 st['scales'].data_ptr() if 'scales' in st else 0, st['step'].data_ptr(), p.numel())])
             self.tables.append(table)
-            self.sets.append((at, dtype_code(dtype), bits, first, len(rs), _address(table)))
+            self.sets.append((at, dtype_code(dtype), first, len(rs), _address(table)))
             first += len(rs)
-        self.words = [2 * first, 2 * first + sum(int(fn['unetk_grad_partials'](s[4])) for s in self.sets)]
+        self.words = [2 * first, 2 * first + sum(int(fn['unetk_grad_partials'](s[3])) for s in self.sets)]
         self.state = list(opt.state.values())
         self.kept = list(chain.from_iterable(map(dict.values, self.state)))
         self.where = list(map(_get_pointer, self.params)) + list(map(_get_pointer, self.kept))

@@ -35,8 +35,8 @@ def test_entry_points_refuse_before_launch(nat):
         return fn['unetk_adamw_prepare'](a(t) if t else None, a(g) if g else None, n, dtype, 1e-3, None, 0.9, 0.999, 0.0, 0, None,
                                          coefs, partials, None)
 
-    def update(name, t=good, g=grad, n=1, dtype=nat.F32, coefs=64, partials=None, count=0, max_norm=1.0):
-        return fn[name](a(t) if t else None, a(g) if g else None, n, dtype, 0.9, 0.999, 1e-8, None, None, coefs, partials, count,
+    def update(t=good, g=grad, n=1, dtype=nat.F32, coefs=64, partials=None, count=0, max_norm=1.0):
+        return fn['unetk_adamw_update'](a(t) if t else None, a(g) if g else None, n, dtype, 0.9, 0.999, 1e-8, None, None, coefs, partials, count,
                         max_norm, None, None)
 
     assert prepare(None) == -5 and prepare(g=None) == -5 and prepare(n=0) == -5 and prepare(dtype=9) == -2
@@ -44,21 +44,22 @@ def test_entry_points_refuse_before_launch(nat):
     assert prepare(words(*ROW[:4], 0, 10)) == -5 and prepare(words(*ROW[:4], 66, 10)) == -3            # step
     assert prepare(words(*ROW[:5], -1)) == -5 and prepare(words(*ROW[:5], 1 << 60)) == -1              # numel
     assert prepare(g=words(0)) == -5 and prepare(g=words(66)) == -3
-    for name in ('unetk_adamw_update', 'unetk_adamw8_update'):
-        assert update(name, None) == -5 and update(name, g=None) == -5 and update(name, n=-1) == -5 and update(name, dtype=3) == -2
-        assert update(name, coefs=None) == -5
-        assert update(name, partials=64, count=0) == -5 and update(name, partials=None, count=4) == -5
-        assert update(name, partials=12, count=4) == -3
+    for scales in (0, 64):
+        row = (*ROW[:3], scales, *ROW[4:])
+        assert update(None) == -5 and update(g=None) == -5 and update(n=-1) == -5 and update(dtype=3) == -2
+        assert update(coefs=None) == -5
+        assert update(partials=64, count=0) == -5 and update(partials=None, count=4) == -5
+        assert update(partials=12, count=4) == -3
         for bad in (-1.0, float('nan')):
-            assert update(name, partials=64, count=4, max_norm=bad) == -5
+            assert update(partials=64, count=4, max_norm=bad) == -5
         for k in range(3):
-            r = list(ROW)
+            r = list(row)
             r[k] = 0
-            assert update(name, words(*r)) == -5
-        assert update(name, g=words(0)) == -5
-        assert update(name, words(*ROW, 66, *ROW[1:]), words(64, 64), 2) == -3                         # an fp32 parameter at two bytes
-    assert update('unetk_adamw8_update', words(*ROW[:3], 0, *ROW[4:])) == -5
-    assert fn['unetk_grad_partials'](0) == -5 and fn['unetk_grad_partials'](65) == 2 * fn['unetk_grad_partials'](64)
+            assert update(words(*r)) == -5
+        assert update(g=words(0)) == -5
+        assert update(words(*row, 66, *row[1:]), words(64, 64), 2) == -3                         # an fp32 parameter at two bytes
+    assert update(words(64, 66, 64, 0, 64, 10)) == -3 and update(words(64, 64, 66, 0, 64, 10)) == -3       # fp32 moments at two bytes
+    assert fn['unetk_grad_partials'](0) == -5 and 0 < fn['unetk_grad_partials'](1) <= fn['unetk_grad_partials'](1000)
     ten = words(10)
     assert fn['unetk_grad_sumsq'](a(grad), a(ten), 1, nat.F32, None, None) == -5
     assert fn['unetk_grad_sumsq'](a(grad), a(ten), 1, nat.F32, 12, None) == -3

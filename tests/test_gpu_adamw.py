@@ -94,7 +94,7 @@ def check_step(params, before, after, hyper, max_norm=None, seed=0, total_norm=N
 
 SIZES = {'one': [1], 'small': [3, 1, 2, 255, 256, 257], 'edges': [4095, 4096, 4097, 8191, 12288 + 1], 'mixed': [100003, 7, 4096, 65537, 64],
          'many': [1 + (37 * i) % 700 for i in range(64)], 'more': [1 + (53 * i) % 500 for i in range(65)],
-         'lots': [1 + (29 * i) % 300 for i in range(200)]}
+         'lots': [1 + (29 * i) % 300 for i in range(200)], 'most': [(31 * i) % 90 for i in range(385)] + [9001]}
 
 
 @pytest.mark.parametrize('sizes', list(SIZES))
