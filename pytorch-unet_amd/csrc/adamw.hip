@@ -10,6 +10,7 @@ namespace {
 
 constexpr int kGrads = 192;       // tensors a launch that needs their gradients alone: 20 bytes each
 constexpr int kPrepare = 128;     // 28 bytes each
+constexpr int kSteps = 256;       // a prepare without sums: 8 bytes and a thread each
 constexpr int kUpdate = 64;       // 52 bytes each
 constexpr int kChunk = 4096;      // elements: 16 per thread
 constexpr int kBlock = 256;       // elements that share a scale: one wave, four per lane
@@ -26,6 +27,9 @@ template <int N> struct Chunks {
 struct GradTable {
   Chunks<kGrads> c;
   void* grad[kGrads];
+};
+struct StepTable {
+  float* step[kSteps];
 };
 struct PrepareTable {
   Chunks<kPrepare> c;
@@ -166,25 +170,33 @@ __device__ __forceinline__ unsigned mix32(unsigned h) {
   return h ^ (h >> 16);
 }
 
-// Counts the step and writes the bias corrections (workgroup 0, a thread per tensor); with SUM also the partial sums.
-template <typename T, bool SUM>
-__global__ __launch_bounds__(256) void adamw_prepare_kernel(PrepareTable tb, int n_tensors, double lr,
-                                                            const float* __restrict__ lr_dev, double beta1, double beta2,
-                                                            double weight_decay, unsigned seed,
-                                                            const float* __restrict__ found_inf, Coefs* __restrict__ coefs,
+struct Schedule {
+  double lr, beta1, beta2, weight_decay;
+  const float* lr_dev;
+  const float* found_inf;
+  unsigned seed;
+};
+// Counts a tensor's step and writes its bias corrections.
+__device__ __forceinline__ void count_step(float* step, const Schedule& h, Coefs* out) {
+  if (h.found_inf && *h.found_inf != 0.f) return;
+  const float t = *step + 1.f;
+  *step = t;
+  const double rate = h.lr_dev ? (double)*h.lr_dev : h.lr;
+  Coefs c;
+  c.step_size = (float)(rate / (1.0 - pow(h.beta1, (double)t)));
+  c.root_correction = (float)(1.0 / sqrt(1.0 - pow(h.beta2, (double)t)));
+  c.decay = (float)(1.0 - rate * h.weight_decay);
+  c.key = mix32((unsigned)(long)t * 0x9E3779B9u + h.seed);
+  *out = c;
+}
+__global__ __launch_bounds__(kSteps) void adamw_steps_kernel(StepTable tb, int n_tensors, Schedule h, Coefs* __restrict__ coefs) {
+  if (threadIdx.x < n_tensors) count_step(tb.step[threadIdx.x], h, coefs + threadIdx.x);
+}
+template <typename T>
+__global__ __launch_bounds__(256) void adamw_prepare_kernel(PrepareTable tb, int n_tensors, Schedule h, Coefs* __restrict__ coefs,
                                                             double* __restrict__ partials) {
-  if (blockIdx.x == 0 && threadIdx.x < n_tensors && !(found_inf && *found_inf != 0.f)) {
-    const float t = *tb.step[threadIdx.x] + 1.f;
-    *tb.step[threadIdx.x] = t;
-    const double rate = lr_dev ? (double)*lr_dev : lr;
-    Coefs c;
-    c.step_size = (float)(rate / (1.0 - pow(beta1, (double)t)));
-    c.root_correction = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)t)));
-    c.decay = (float)(1.0 - rate * weight_decay);
-    c.key = mix32((unsigned)(long)t * 0x9E3779B9u + seed);
-    coefs[threadIdx.x] = c;
-  }
-  if constexpr (SUM) write_partial<T>(tb, partials);
+  if (blockIdx.x == 0 && threadIdx.x < n_tensors) count_step(tb.step[threadIdx.x], h, coefs + threadIdx.x);
+  write_partial<T>(tb, partials);
 }
 
 // What the gradient is multiplied by.  Every workgroup sums the partials in the same order, so all agree to the bit.  A norm that is
@@ -541,7 +553,7 @@ int unetk_grad_clip(void* const* grads, const int64_t* numel, int n_tensors, int
   if (rc == UNETK_OK) rc = check_clip(partials, n_partials, max_norm);
   if (rc != UNETK_OK) return rc;
   if (!partials) return UNETK_ERR_ARG;
-  for (int at = 0; at < n_tensors; at += kGrads) {
+  for (int at = (n_tensors - 1) / kGrads * kGrads; at >= 0; at -= kGrads) {
     const int n = part_of(n_tensors, at, kGrads);
     GradTable tb;
     if (!fill_chunks(n, &tb.c, [&](int i) { return numel[at + i]; })) return UNETK_ERR_SHAPE;
@@ -561,24 +573,29 @@ int64_t unetk_adamw_prepare(const unetk_adamw_tensor* tensors, void* const* grad
   if (rc != UNETK_OK) return rc;
   if (!coefs) return UNETK_ERR_ARG;
   if (((uintptr_t)partials & 7) || ((uintptr_t)coefs & 15)) return UNETK_ERR_ALIGN;
+  const Schedule h{lr, beta1, beta2, weight_decay, lr_dev, found_inf, (unsigned)seed};
+  if (!partials) {
+    for (int at = 0; at < n_tensors; at += kSteps) {
+      const int n = part_of(n_tensors, at, kSteps);
+      StepTable tb;
+      for (int i = 0; i < n; ++i) tb.step[i] = tensors[at + i].step;
+      hipLaunchKernelGGL(adamw_steps_kernel, dim3(1), dim3(kSteps), 0, (hipStream_t)stream, tb, n, h,
+                         reinterpret_cast<Coefs*>(coefs) + at);
+      UNETK_CHECK_LAUNCH();
+    }
+    return 0;
+  }
   int64_t written = 0;
   for (int at = 0; at < n_tensors; at += kPrepare) {
     const int n = part_of(n_tensors, at, kPrepare);
     PrepareTable tb;
     if (!fill_chunks(n, &tb.c, [&](int i) { return tensors[at + i].numel; })) return UNETK_ERR_SHAPE;
     for (int i = 0; i < n; ++i) tb.grad[i] = grads[at + i], tb.step[i] = tensors[at + i].step;
-    Coefs* co = reinterpret_cast<Coefs*>(coefs) + at;
-    if (partials) {
-      const int grid = grid_of(tb.c.total, kSumsqGrid);
-      UNETK_WITH_T(dtype, hipLaunchKernelGGL((adamw_prepare_kernel<T, true>), dim3(grid), dim3(256), 0, (hipStream_t)stream, tb, n,
-                                             lr, lr_dev, beta1, beta2, weight_decay, (unsigned)seed, found_inf, co,
-                                             partials + written));
-      written += grid;
-    } else {
-      hipLaunchKernelGGL((adamw_prepare_kernel<float, false>), dim3(1), dim3(256), 0, (hipStream_t)stream, tb, n, lr, lr_dev,
-                         beta1, beta2, weight_decay, (unsigned)seed, found_inf, co, (double*)nullptr);
-    }
+    const int grid = grid_of(tb.c.total, kSumsqGrid);
+    UNETK_WITH_T(dtype, hipLaunchKernelGGL(adamw_prepare_kernel<T>, dim3(grid), dim3(256), 0, (hipStream_t)stream, tb, n, h,
+                                           reinterpret_cast<Coefs*>(coefs) + at, partials + written));
     UNETK_CHECK_LAUNCH();
+    written += grid;
   }
   return written;
 }
@@ -592,7 +609,7 @@ int unetk_adamw_update(const unetk_adamw_tensor* tensors, void* const* grads, in
   if (!coefs) return UNETK_ERR_ARG;
   const Betas b{(float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps};
   const Clip clip{partials, (int)n_partials, (float)max_norm, grad_scale, norm_out};
-  for (int at = 0; at < n_tensors; at += kUpdate) {
+  for (int at = (n_tensors - 1) / kUpdate * kUpdate; at >= 0; at -= kUpdate) {
     const int n = part_of(n_tensors, at, kUpdate);
     Update8Table tb;
     if (!fill_update(tensors + at, grads + at, n, &tb)) return UNETK_ERR_SHAPE;

@@ -535,7 +535,7 @@ class _Plan:
                 return None
             if not all(map(_get_contiguous, grads)) if self.contiguous else list(map(_get_stride, grads)) != self.strides:
                 return None
-            return array('q', map(_get_pointer, grads))
+            return array('q', list(map(_get_pointer, grads)))
         except (TypeError, RuntimeError):                # a gradient that is None, or not a strided tensor
             return None
 
