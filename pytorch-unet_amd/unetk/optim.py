@@ -12,6 +12,7 @@ buffer of unetk.ddp.FlatGrads, the optimizer state is two more flat buffers, and
 (or the flat buffers above), decoupled weight decay, moments in 32 or in 8 bits, the clip in front of the step or by itself.
 """
 import contextlib
+import weakref
 from array import array
 from itertools import chain
 from operator import is_
@@ -152,7 +153,7 @@ _TYPES = {torch.float32, torch.bfloat16, torch.float16}
 # one C call per tensor each: a step of small tensors is bound by what the host asks of them
 _get_pointer, _get_numel, _get_device = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device
 _get_contiguous, _get_dtype, _get_stride = torch.Tensor.is_contiguous, torch.Tensor.dtype.__get__, torch.Tensor.stride
-_get_wanted = torch.Tensor.requires_grad.__get__
+_get_wanted, _get_referent = torch.Tensor.requires_grad.__get__, weakref.ref.__call__
 
 
 def _address(words):
@@ -237,6 +238,11 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     return norm
 
 
+def _not_captured(what):
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f'AdamW: take one step before capturing: a graph cannot {what}, every replay would do it again')
+
+
 def _written(count, what):
     if count < 0:
         check(int(count), what)
@@ -289,10 +295,6 @@ class AdamW(torch.optim.Optimizer):
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_norm=None, state_bits=32,
                  min_8bit_numel=4096, seed=0):
         self.fg = params if hasattr(params, 'module_order') else None
-        if not isinstance(lr, torch.Tensor) and not lr >= 0:
-            raise ValueError(f'AdamW: lr must not be negative, got {lr}')
-        if not eps >= 0 or not weight_decay >= 0:
-            raise ValueError(f'AdamW: eps and weight_decay must not be negative, got {eps}, {weight_decay}')
         if state_bits not in (8, 32):
             raise ValueError(f'AdamW: state_bits must be 8 or 32, got {state_bits}')
         self.state_bits, self.min_8bit_numel, self.seed = state_bits, int(min_8bit_numel), int(seed) & 0xFFFFFFFF
@@ -316,16 +318,29 @@ class AdamW(torch.optim.Optimizer):
     def _check_group(self, g):
         if len({id(p) for p in g['params']}) != len(g['params']):
             raise ValueError('AdamW: a parameter appears twice')
+        for k in ('lr', 'eps', 'weight_decay'):
+            if not isinstance(g[k], torch.Tensor) and not g[k] >= 0:
+                raise ValueError(f'AdamW: {k} must not be negative, got {g[k]}')
         if not all(0.0 <= b < 1.0 for b in g['betas']):
             raise ValueError(f"AdamW: betas must lie in [0, 1), got {g['betas']}")
         if g['max_norm'] is not None and not g['max_norm'] > 0:
             raise ValueError(f"AdamW: max_norm must be positive or None, got {g['max_norm']}")
         if g['max_norm'] != self.param_groups[0]['max_norm']:
             raise ValueError('AdamW: the clip is over all groups: max_norm must be the same in each')
+        if self.fg is not None and not all(id(p) in self.fg.offsets for p in g['params']):
+            raise ValueError('AdamW: a parameter has no place in the flat gradient buffer')
         for p in g['params']:
             _require(p, 'parameters')
             if p.device != next(q for h in self.param_groups for q in h['params']).device:
                 raise RuntimeError('AdamW: parameters must be on one device')
+
+    def __getstate__(self):
+        return {**super().__getstate__(), 'fg': self.fg, 'state_bits': self.state_bits, 'min_8bit_numel': self.min_8bit_numel,
+                'seed': self.seed, 'total_norm': self.total_norm}
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._plan = None
 
     def zero_grad(self, set_to_none=True):
         if self.fg is not None:
@@ -334,9 +349,7 @@ class AdamW(torch.optim.Optimizer):
 
     # ---- state
     def _new_state(self, p):
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError('AdamW: take one step (or load a state) before capturing: state made inside a graph would be '
-                               'cleared by every replay')
+        _not_captured('make its state')
         st = {'step': torch.zeros((), dtype=torch.float32, device=p.device)}
         if self.state_bits == 8 and p.numel() >= self.min_8bit_numel:
             for k in ('exp_avg', 'exp_avg_root'):
@@ -365,6 +378,7 @@ class AdamW(torch.optim.Optimizer):
                     sc.device != p.device:
                 raise RuntimeError("AdamW: state 'scales' must be contiguous float8_e8m0fnu [ceil(numel / 256), 2]")
         if any(st[k].stride() != p.stride() for k in names):
+            _not_captured('lay its state out anew')
             st.update(_fit_moments(p, st, bits))
         return bits
 
@@ -388,9 +402,13 @@ class AdamW(torch.optim.Optimizer):
             state[p] = _fit_moments(p, st, bits)
             state[p]['step'] = torch.tensor(float(st['step']), dtype=torch.float32, device=p.device)
         for own, g in zip(self.param_groups, groups):
-            for k in ('lr', 'betas', 'eps', 'weight_decay', 'max_norm', 'initial_lr'):
+            for k in ('betas', 'eps', 'weight_decay', 'max_norm', 'initial_lr'):
                 if k in g:
                     own[k] = g[k]
+            if isinstance(own['lr'], torch.Tensor):      # a captured graph reads this very tensor
+                own['lr'].fill_(float(g['lr']))
+            else:
+                own['lr'] = float(g['lr'])
         self._plan = None
         self.state.clear()
         self.state.update(state)
@@ -405,13 +423,14 @@ class AdamW(torch.optim.Optimizer):
             raise RuntimeError('AdamW.step: no gradients (run backward through the UNet first)')
         plan = self._plan
         pointers = plan.pointers(self) if plan is not None else None
-        if pointers is None:                             # the first step, or something moved, came or went
-            plan = self._plan = None
-            with torch.no_grad():
-                plan, pointers, copies = self._make_plan()
-        if plan.params:
-            with _on_device(plan.device):
+        with _on_device(next(p.device for g in self.param_groups for p in g['params'])):
+            if pointers is None:                         # the first step, or something moved, came or went
+                plan = self._plan = None
+                with torch.no_grad():
+                    plan, pointers, copies = self._make_plan()
+            if plan.params:
                 self._launch(plan, pointers)
+        if plan.params:
             # the kernels wrote the parameters behind PyTorch's back: bump their version counters like any in-place op
             torch.autograd.graph.increment_version(plan.params)
         self._plan = plan
@@ -431,6 +450,7 @@ class AdamW(torch.optim.Optimizer):
                     absent.append(p)
                     continue
                 if self.fg is not None and not p.is_contiguous():
+                    _not_captured('lay its parameters out anew')
                     p.data = p.data.contiguous()
                 _require(p, 'parameters')
                 st = self.state.get(p)
@@ -485,7 +505,8 @@ class AdamW(torch.optim.Optimizer):
 
 class _Plan:
     """What one step found out about its tensors, for the next one: everything but the gradients' pointers, and how to tell that
-    it still holds.  It keeps the tensors it speaks of alive, so an address in it cannot become another tensor's."""
+    it still holds.  It does not keep the state alive (a user may move that off the device between steps): references tell
+    whether a tensor is the same one, its address whether it is where it was."""
 
     def __init__(self, opt, sets, absent):
         rows = [r for rs in sets.values() for r in rs]
@@ -503,8 +524,9 @@ class _Plan:
             first += len(rs)
         self.words = [2 * first, 2 * first + sum(int(fn['unetk_grad_partials'](s[3])) for s in self.sets)]
         self.state = list(opt.state.values())
-        self.kept = list(chain.from_iterable(map(dict.values, self.state)))
-        self.where = list(map(_get_pointer, self.params)) + list(map(_get_pointer, self.kept))
+        tensors = list(chain.from_iterable(map(dict.values, self.state)))
+        self.refs = list(map(weakref.ref, tensors))
+        self.where = list(map(_get_pointer, self.params)) + list(map(_get_pointer, tensors))
         self.types, self.numel = list(map(_get_dtype, self.params)), list(map(_get_numel, self.params))
         self.contiguous = all(map(_get_contiguous, self.params))
         self.strides = None if self.contiguous else list(map(_get_stride, self.params))
@@ -518,7 +540,9 @@ class _Plan:
         if [len(g['params']) for g in opt.param_groups] != self.counts or len(now) != len(self.state) or \
                 not all(map(is_, now, self.state)):
             return None
-        if list(map(_get_pointer, params)) + list(map(_get_pointer, chain.from_iterable(map(dict.values, now)))) != self.where:
+        tensors = list(chain.from_iterable(map(dict.values, now)))
+        if len(tensors) != len(self.refs) or not all(map(is_, tensors, map(_get_referent, self.refs))) or \
+                list(map(_get_pointer, params)) + list(map(_get_pointer, tensors)) != self.where:
             return None
         if not all(map(_get_contiguous, params)) if self.contiguous else list(map(_get_stride, params)) != self.strides:
             return None

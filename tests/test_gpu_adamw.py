@@ -89,7 +89,10 @@ def check_step(params, before, after, hyper, max_norm=None, seed=0, total_norm=N
                 assert lo <= kk <= hi
             lo, hi = O.code_range(x, xe, k, u, root)
             assert (lo <= codes).all() and (codes <= hi).all()
-            assert (lo == hi).mean() > 0.99 or len(lo) < 1000       # the bound leaves a choice at almost no element
+            # the bound leaves a choice at almost no element -- but where a square falls among fp32's subnormals, whose root may
+            # be off by 2^-74 and so be anything among the smallest
+            clear = xe <= 1e-6 * np.abs(x)
+            assert clear.sum() < 1000 or (lo == hi)[clear].mean() > 0.99
 
 
 SIZES = {'one': [1], 'small': [3, 1, 2, 255, 256, 257], 'edges': [4095, 4096, 4097, 8191, 12288 + 1], 'mixed': [100003, 7, 4096, 65537, 64],
@@ -253,6 +256,22 @@ def test_8bit_rounding_does_not_freeze_the_second_moment(optim):
     assert float(root.min()) > 0
 
 
+@pytest.mark.parametrize('bits', [32, 8])
+def test_gradients_of_any_magnitude(optim, bits):
+    """Blocks of 1e-30 (squares vanish) to 1e17 (the largest whose square fp32 holds in v), zeros among them."""
+    mags = [1e-30, 1e-24, 1e-22, 3e-20, 1e-18, 1e-12, 1.0, 1e9, 1e17]
+    g = torch.Generator().manual_seed(11)
+    p = torch.nn.Parameter(torch.randn(256 * len(mags), generator=g).cuda())
+    opt = optim.AdamW([p], **HYPER, state_bits=bits, min_8bit_numel=1)
+    for _ in range(3):
+        grad = torch.randn(len(mags), 256, generator=g) * torch.tensor(mags, dtype=torch.float64)[:, None]
+        grad[:, ::5] = 0.0
+        p.grad = grad.float().view(-1).cuda()
+        before = snapshot(opt, [p])
+        opt.step()
+        check_step([p], before, snapshot(opt, [p]), HYPER)
+
+
 # ------------------------------------------------------------------------------------------ layouts, streams, graphs
 @pytest.mark.parametrize('bits', [32, 8])
 def test_channels_last_parameters_and_a_change_of_layout(optim, bits):
@@ -314,6 +333,15 @@ def test_a_captured_step_counts_and_follows_the_learning_rate(optim, bits):
     with torch.cuda.graph(graph):
         opt.step()
     norm = opt.total_norm
+    if bits == 32:                                                    # what a replay would do over and over is refused
+        w = torch.nn.Parameter(torch.randn(8, 8, 3, 3, device='cuda'))
+        w.grad = torch.randn_like(w)
+        other = optim.AdamW([w])
+        other.step()
+        w.data = w.data.to(memory_format=torch.channels_last)
+        with pytest.raises(RuntimeError, match='before capturing'):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                other.step()
     with torch.cuda.graph(scratch):                                   # another graph's scratch is its own
         optim.clip_grad_norm_(twin, 1e9)
     for k in range(4):
@@ -408,6 +436,10 @@ def test_32bit_checkpoints_are_torchs(optim):
         third.load_state_dict(bad)
     with pytest.raises(ValueError, match='groups'):
         optim.AdamW(c[:1], **kw).load_state_dict(sd)
+    lr = torch.tensor(7.0, device='cuda')                 # the tensor that a graph reads stays that tensor
+    fourth = optim.AdamW(c, lr=lr)
+    fourth.load_state_dict(sd)
+    assert fourth.param_groups[0]['lr'] is lr and abs(float(lr) - kw['lr']) < 1e-9
 
 
 def test_8bit_checkpoints_resume_to_the_bit_and_convert(optim, tmp_path):
@@ -438,6 +470,46 @@ def test_8bit_checkpoints_resume_to_the_bit_and_convert(optim, tmp_path):
     assert all(torch.equal(p, q) for p, q in zip(a, b))
     for k in ('exp_avg', 'exp_avg_root', 'scales'):
         assert torch.equal(oa.state[a[1]][k].view(torch.uint8), ob.state[b[1]][k].view(torch.uint8))
+
+
+def test_copies_of_the_optimizer_and_a_state_that_leaves_the_device(optim):
+    a = make([300, 70001], torch.float32)
+    oa = optim.AdamW(a, **HYPER, state_bits=8, seed=3, max_norm=0.5)
+    oa.step()
+    b, ob = copy.deepcopy((a, oa))
+    for p, q in zip(a, b):
+        q.grad = p.grad
+    c, oc = copy.deepcopy((a, oa))
+    for p, q in zip(a, c):
+        q.grad = p.grad
+    oc.step()
+    for st in oc.state.values():                          # offloaded between steps: the memory is really free, the step refused
+        for k in list(st):
+            st[k] = st[k].cpu()
+    freed = torch.cuda.memory_allocated()
+    with pytest.raises(RuntimeError, match='state'):
+        oc.step()
+    assert torch.cuda.memory_allocated() == freed
+    for st in oc.state.values():
+        for k in list(st):
+            st[k] = st[k].cuda()
+    oa.step(), ob.step(), oa.step(), ob.step(), oc.step()
+    for p, q, r in zip(a, b, c):
+        assert torch.equal(p, q) and torch.equal(p, r)
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason='one GPU')
+def test_parameters_on_another_device_than_the_current_one(optim):
+    p = make([5000, 40], torch.float32)
+    q = [torch.nn.Parameter(x.detach().to('cuda:1')) for x in p]
+    for x, y in zip(p, q):
+        y.grad = x.grad.to('cuda:1')
+    op, oq = optim.AdamW(p, **HYPER, max_norm=0.1, state_bits=8), optim.AdamW(q, **HYPER, max_norm=0.1, state_bits=8)
+    for _ in range(2):
+        op.step(), oq.step()
+    assert float(optim.clip_grad_norm_(p, 0.01)) == float(optim.clip_grad_norm_(q, 0.01))
+    for x, y in zip(p, q):
+        assert torch.equal(x.cpu(), y.cpu()) and torch.equal(x.grad.cpu(), y.grad.cpu())
 
 
 # --------------------------------------------------------------------------------------------------------- refusals
@@ -666,6 +738,8 @@ def test_frozen_parameters_of_a_flat_buffer_stay(optim):
     opt = optim.AdamW(fg, lr=1e-2, weight_decay=0.5)
     with pytest.raises(RuntimeError, match='no gradients'):
         opt.step()
+    with pytest.raises(ValueError, match='no place'):
+        opt.add_param_group({'params': make([10], torch.float32)})
     frozen = net.inc.double_conv[0].weight
     for k in range(4):
         frozen.requires_grad_(k == 2)
