@@ -153,6 +153,7 @@ _TYPES = {torch.float32, torch.bfloat16, torch.float16}
 # one C call per tensor each: a step of small tensors is bound by what the host asks of them
 _get_pointer, _get_numel, _get_device = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device
 _get_contiguous, _get_dtype, _get_stride = torch.Tensor.is_contiguous, torch.Tensor.dtype.__get__, torch.Tensor.stride
+_get_shape = torch.Tensor.shape.__get__
 _get_wanted, _get_referent = torch.Tensor.requires_grad.__get__, weakref.ref.__call__
 
 
@@ -441,7 +442,7 @@ class AdamW(torch.optim.Optimizer):
     def _make_plan(self):
         """Looks every tensor over: the plan of this step, the gradients' pointers, and copies of gradients that lie unlike their
         parameters (to be kept until the launch)."""
-        sets, absent, copies = {}, [], []
+        rows, absent, copies, state = [], [], [], self.state
         for at, group in enumerate(self.param_groups):
             for p in group['params']:
                 # the flat buffer has room for frozen parameters too
@@ -452,19 +453,24 @@ class AdamW(torch.optim.Optimizer):
                 if self.fg is not None and not p.is_contiguous():
                     _not_captured('lay its parameters out anew')
                     p.data = p.data.contiguous()
-                _require(p, 'parameters')
-                st = self.state.get(p)
+                st = state.get(p)
                 if not st:
-                    st = self.state[p] = self._new_state(p)
+                    _require(p, 'parameters')
+                    st = state[p] = self._new_state(p)
+                rows.append((at, p, st, g))
+        if rows and not _all_usual(rows):
+            for k, (at, p, st, g) in enumerate(rows):
+                _require(p, 'parameters')
                 self._check_state(p, st)
                 if g.layout != torch.strided or g.dtype != p.dtype or g.device != p.device or g.shape != p.shape:
                     raise RuntimeError("AdamW: a gradient must be a strided tensor of its parameter's type, shape and device")
                 if g.stride() != p.stride():
-                    g = torch.empty_like(p).copy_(g)
-                    copies.append(g)
-                sets.setdefault((at, p.dtype), []).append((p, st, g))
-        plan = _Plan(self, sets, absent)
-        return plan, array('q', [g.data_ptr() for rows in sets.values() for _, _, g in rows]), copies
+                    copies.append(torch.empty_like(p).copy_(g))
+                    rows[k] = at, p, st, copies[-1]
+        sets = {}
+        for at, p, st, g in rows:
+            sets.setdefault((at, p.dtype), []).append((p, st, g))
+        return _Plan(self, sets, absent), array('q', [g.data_ptr() for rs in sets.values() for _, _, g in rs]), copies
 
     def _launch(self, plan, pointers):
         stream, device = stream_ptr(), plan.device
@@ -501,6 +507,30 @@ class AdamW(torch.optim.Optimizer):
             check(fn['unetk_adamw_update'](table, grads + 8 * first, n, code, *group['betas'], group['eps'], scale_ptr, found_ptr,
                                            coefs + 16 * first, partials, count, max_norm or 0.0, norm_ptr, stream),
                   'unetk_adamw_update')
+
+
+def _all_usual(rows):
+    """What nearly every step finds, looked at attribute by attribute for all tensors together: everything contiguous, of the
+    right types and shapes, on one device.  False leaves it to the checks of each tensor, which say what is wrong."""
+    _, params, states, grads = zip(*rows)
+    try:
+        wide = [(p, st) for p, st in zip(params, states) if 'scales' not in st]
+        code = [(p, st) for p, st in zip(params, states) if 'scales' in st]
+        like = list(params) * 3
+        moments = [st['exp_avg'] for st in states] + [st['exp_avg_root' if 'scales' in st else 'exp_avg_sq'] for st in states]
+        steps, scales = [st['step'] for st in states], [st['scales'] for _, st in code]
+        every = [*params, *grads, *moments, *scales]
+        return (all(map(_get_contiguous, every))
+                and len(set(map(_get_device, [*every, *steps]))) == 1 and params[0].is_cuda
+                and list(map(_get_dtype, params)) == list(map(_get_dtype, grads)) and set(map(_get_dtype, params)) <= _TYPES
+                and list(map(_get_shape, like)) == list(map(_get_shape, [*grads, *moments]))
+                and {st[k].dtype for _, st in wide for k in ('exp_avg', 'exp_avg_sq')} <= {torch.float32}
+                and {st[k].dtype for _, st in code for k in ('exp_avg', 'exp_avg_root')} <= {_CODE}
+                and set(map(_get_dtype, steps)) == {torch.float32} and set(map(_get_numel, steps)) == {1}
+                and set(map(_get_dtype, scales)) <= {_SCALE}
+                and all(tuple(st['scales'].shape) == (-(-p.numel() // BLOCK), 2) for p, st in code))
+    except (KeyError, AttributeError, TypeError, RuntimeError):
+        return False
 
 
 class _Plan:
