@@ -4,6 +4,16 @@
 // The tensors of a call travel as kernel arguments, a table of up to 4 KiB a launch: nothing is uploaded, kept or shared between
 // calls, and a captured graph owns its copy.  Each tensor is cut into chunks of kChunk elements; a workgroup takes every
 // gridDim.x-th chunk and finds its tensor with one compare per lane and a ballot over 64 tensors' first chunks.
+//
+// Everything here is bound by HBM (a copy of 2 GB reaches 5.0 TB/s on this card, a sum 4.0 to 6.3).  Measured, three sets of
+// inputs in turn so that no step finds its own in the 256 MiB last-level cache; "U-Net": 31 M elements in 64 tensors, "wide":
+// 124 M; bytes are what a step has to read and write once, the second read of the gradients not counted:
+//                                   sums + counts    update                whole step
+//   fp32, clip, U-Net                  21.5 us       139 us, 6.2 TB/s      161 us   (0.87 GB, 174 us at the copy's rate)
+//   fp32, clip, wide                   80            594,    5.9           675      (3.48 GB, 695)
+//   bf16, clip, 17 M elements           8.8           67,    5.7            76      (0.38 GB, 76)
+//   8-bit moments, fp32, U-Net         23             75,    6.6            98      (0.50 GB, 99)
+//   8-bit moments, bf16, wide          41            212,    5.9           254      (1.24 GB, 249)
 #include "common.h"
 
 namespace {
@@ -12,11 +22,15 @@ constexpr int kGrads = 192;       // tensors a launch that needs their gradients
 constexpr int kPrepare = 128;     // 28 bytes each
 constexpr int kSteps = 256;       // a prepare without sums: 8 bytes and a thread each
 constexpr int kUpdate = 64;       // 52 bytes each
-constexpr int kChunk = 4096;      // elements: 16 per thread
+constexpr int kChunk = 4096;      // elements, 16 per thread; 2048 / 8192: wide 738 / 723 us (724), 190 tensors 52 / 61 us (54)
 constexpr int kBlock = 256;       // elements that share a scale: one wave, four per lane
+// Workgroups at most.  The sums: 512 / 1024 / 2048 read 118 MiB in 23.8 / 21.8 / 22.4 us, and every later workgroup adds up that
+// many partials.  The clip does not mind (512 to 4096: +-1 %).  The update wants few streams at once, 512 / 768 / 1024 / 2048
+// take 166 / 163 / 165 / 169 us for the U-Net and 662 / 676 / 685 / 724 for its wide form, 83 / 76 / 77 / 81 in bf16.  The 8-bit
+// one has arithmetic to hide and evens out its end with many: 2048 / 4096 / 8192 take 102.5 / 98.5 / 97.9 and 293 / 292 / 274 us.
 constexpr int kSumsqGrid = 1024;
 constexpr int kClipGrid = 2048;
-constexpr int kUpdateGrid = 768;  // three workgroups per CU
+constexpr int kUpdateGrid = 768;
 constexpr int kUpdate8Grid = 8192;
 
 template <int N> struct Chunks {
@@ -58,7 +72,8 @@ struct Coefs {                    // per tensor, written by the prepare kernel
   float step_size, root_correction, decay;
   unsigned key;
 };
-static_assert(sizeof(GradTable) <= 3900 && sizeof(PrepareTable) <= 3900 && sizeof(Update8Table) <= 3900, "with a launch's scalars under 4 KiB");
+static_assert(sizeof(GradTable) <= 3900 && sizeof(PrepareTable) <= 3900 && sizeof(Update8Table) <= 3900,
+              "with a launch's scalars under 4 KiB");
 static_assert(kGrads % 64 == 0 && kPrepare % 64 == 0 && kPrepare <= 256 && kUpdate % 64 == 0, "lanes and threads");
 static_assert(sizeof(Coefs) == 16, "unetk.h promises 16 bytes a tensor");
 
@@ -85,8 +100,11 @@ typedef unsigned short u16u __attribute__((aligned(1)));
 template <typename T> struct Raw4 { typedef u16x4u type; };
 template <> struct Raw4<float> { typedef f32x4u type; };
 
-// FULL: all four exist; otherwise those before n, zeros behind.  ONCE: nothing of this step reads them again.
-template <typename T, bool FULL, bool ONCE = false> __device__ __forceinline__ typename Raw4<T>::type load4(const void* base, long i, long n) {
+// FULL: all four exist; otherwise those before n, zeros behind.  ONCE: nothing of this step reads them again, so they pass by
+// the caches, as all stores do, and leave the gradients there between the sums and the update: the U-Net's step falls from 195
+// to 172 us, the wide one's from 792 to 727; with the gradients passing by as well it is 181 and 714 instead of 161 and 675.
+template <typename T, bool FULL, bool ONCE = false>
+__device__ __forceinline__ typename Raw4<T>::type load4(const void* base, long i, long n) {
   typedef typename Raw4<T>::type V;
   const T* p = static_cast<const T*>(base) + i;
   if (FULL && ONCE) return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
@@ -147,6 +165,8 @@ template <typename T, bool FULL> __device__ __forceinline__ double chunk_sumsq(c
     }
   return s;
 }
+// One read of the gradients at 5.7 (124 MB) to 6.3 TB/s (1.6 GB); a workgroup's sum goes to a slot of its own, so that the norm
+// does not depend on who comes first.
 template <typename T, typename Table> __device__ __forceinline__ void write_partial(const Table& tb, double* partials) {
   const Owners owners(tb.c);
   double s = 0.0;
@@ -199,7 +219,8 @@ __global__ __launch_bounds__(256) void adamw_prepare_kernel(PrepareTable tb, int
   write_partial<T>(tb, partials);
 }
 
-// What the gradient is multiplied by.  Every workgroup sums the partials in the same order, so all agree to the bit.  A norm that is
+// What the gradient is multiplied by.  Every workgroup sums the partials in the same order, so all agree to the bit, and no
+// launch in between has to (a kernel of one workgroup costs 3 us, these sums under 1).  A norm that is
 // not a number makes the coefficient one that is not either, as clip_grad_norm_ does.
 __device__ __forceinline__ float grad_factor(const Clip& c) {
   const double inv_scale = c.grad_scale ? 1.0 / (double)*c.grad_scale : 1.0;
@@ -214,6 +235,8 @@ __device__ __forceinline__ float grad_factor(const Clip& c) {
   return (float)(coef * inv_scale);
 }
 
+// Second pass of the clip: 39 us for 124 MB of gradients (6.3 TB/s read and written, the read mostly from the last-level cache),
+// from the last chunk the sums read to the first, as in the updates.
 template <typename T, bool FULL> __device__ __forceinline__ void clip_chunk(void* grad, long base, long n, float coef) {
   typename Raw4<T>::type g[kChunk / 1024];
 #pragma unroll
@@ -242,7 +265,8 @@ struct Betas {
   float beta1, rest1, beta2, rest2, eps;
 };
 
-// One element: the moments in place, the new parameter returned.
+// One element: the moments in place, the new parameter returned.  Square root and quotient are the correctly rounded ones: at
+// 28 bytes an element there is time for 200 vector instructions, and this takes about 60.
 __device__ __forceinline__ float adamw_element(float p, float g, float& m, float& v, const Coefs& c, const Betas& b) {
   m = fmaf(b.rest1, g, b.beta1 * m);
   v = fmaf(b.rest2 * g, g, b.beta2 * v);
@@ -271,6 +295,7 @@ __device__ __forceinline__ void update_chunk(const UpdateTable& tb, int t, long 
   }
 }
 
+// From the last chunk to the first: what the sums read last is still in the last-level cache (forwards: up to 3 % more).
 template <typename T>
 __global__ __launch_bounds__(256) void adamw_update_kernel(UpdateTable tb, Betas b, const Coefs* __restrict__ coefs,
                                                            const float* __restrict__ found_inf, Clip clip) {
@@ -335,7 +360,12 @@ template <bool ROOT> __device__ __forceinline__ unsigned encode4_special(const f
   return (encode4<ROOT>(y, *e, carry) & ~nan) | (nan & 0x7f7f7f7fu);
 }
 
-// A block of 256 elements, a wave's.
+// A block of 256 elements, a wave's: four per lane, so that codes move as words, parameters as 8 or 16 bytes, and the block's
+// maxima need six DPP steps and no LDS.  At 10 bytes an element (bf16) HBM leaves time for some 70 vector instructions; with
+// correctly rounded roots and quotients, shuffles and checks at each element it took about 120 (373 us for 124 M elements),
+// now about 60 (212 us, bound by HBM again): the scale's arithmetic is scalar, root and reciprocal are one instruction each
+// (1 ulp, against a rounding to 3 bits of mantissa in the moments and 4 roundings in the update), and values that are not
+// finite or squares that are subnormal (v_sqrt_f32 takes those for zero) are looked for once a wave.
 template <typename T, bool FULL>
 __device__ __forceinline__ void update_block(const Update8Table& tb, int t, long block, long n, float factor, const Coefs& c,
                                              const Betas& b) {
@@ -414,7 +444,8 @@ __device__ __forceinline__ void update_block(const Update8Table& tb, int t, long
   if (lane == 0) *sp = (unsigned short)(me | re << 8);
 }
 
-// Tensors with 8-bit moments and, in the same launch, tensors with fp32 moments (a network's biases and BatchNorms).
+// Tensors with 8-bit moments and, in the same launch, tensors with fp32 moments (a network's biases and BatchNorms: a launch of
+// their own took 7 to 14 us).
 template <typename T>
 __global__ __launch_bounds__(256) void adamw8_update_kernel(Update8Table tb, Betas b, const Coefs* __restrict__ coefs,
                                                             const float* __restrict__ found_inf, Clip clip) {
