@@ -286,6 +286,8 @@ class AdamW(torch.optim.Optimizer):
     element's index, for tensors of at least `min_8bit_numel` elements; smaller ones (biases, BatchNorm) keep 32 bits.
     lr: a float, or an fp32 scalar tensor on the device, which a captured graph reads anew at each replay.
 
+    The rounding is the same on every rank of a data-parallel job.  A parameter that is laid out anew (net.to(memory_format=...))
+    takes its moments along, 8-bit ones rounded to nearest in their new blocks.
     state[p]: `step` (fp32 scalar on the device), `exp_avg`, and `exp_avg_sq` or, in 8 bits, `exp_avg_root` (the square root)
     and `scales`.  With 32 bits state_dict() is torch.optim.AdamW's; load_state_dict() takes that one's and either form.
     Under torch.amp.GradScaler the step is skipped on the device, without a read-back.  A step can be captured into a graph once
@@ -397,6 +399,8 @@ class AdamW(torch.optim.Optimizer):
             if index not in state_dict['state']:
                 continue
             st = state_dict['state'][index]
+            if 'step' not in st or 'exp_avg' not in st or not ('exp_avg_sq' in st or {'exp_avg_root', 'scales'} <= set(st)):
+                raise ValueError('AdamW.load_state_dict: not the state of an AdamW')
             if tuple(st['exp_avg'].shape) != tuple(p.shape):
                 raise ValueError('AdamW.load_state_dict: state shape does not match the parameter')
             bits = 8 if self.state_bits == 8 and p.numel() >= self.min_8bit_numel else 32
@@ -596,6 +600,8 @@ class _Plan:
 
 def _fit_moments(p, st, bits):
     """The moments of a state in the form and memory layout that parameter `p` needs."""
+    if bits == 8 and 'scales' in st and st['exp_avg'].stride() == p.stride():
+        return {k: st[k].view(torch.uint8).to(p.device, copy=True).view(st[k].dtype) for k in ('exp_avg', 'exp_avg_root', 'scales')}
     first, second = (torch.empty_like(p, dtype=torch.float32) for _ in range(2))
     if 'scales' in st:
         sc = st['scales']

@@ -61,13 +61,12 @@ def snapshot(opt, params):
     return rec
 
 
-def check_step(params, before, after, hyper, max_norm=None, seed=0, total_norm=None, grad_scale=1.0):
-    grads = [b['g'] / grad_scale for b in before if b['g'] is not None]
-    factor, err = 1.0 / grad_scale, 0.0
+def check_step(params, before, after, hyper, max_norm=None, seed=0, total_norm=None, norm=None):
+    factor, err = 1.0, 0.0
     if max_norm is not None:
-        norm = O.norm(grads)
+        norm = O.norm([b['g'] for b in before if b['g'] is not None]) if norm is None else norm
         assert abs(float(total_norm) - norm) <= 3 * O.U * norm
-        factor, err = O.clip_coef(norm, max_norm) / grad_scale, COEF_ERR
+        factor, err = O.clip_coef(norm, max_norm), COEF_ERR
     for p, b, a in zip(params, before, after):
         if b['g'] is None:
             assert a['t'] == b['t'] and np.array_equal(a['p'], b['p'])
@@ -132,6 +131,35 @@ def test_no_limit_reached_and_extreme_hyperparameters(optim, bits):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
         if hyper['lr'] == 0.0:
             assert all(torch.equal(x, y) for x, y in zip(a, make([5000, 33], torch.float32)))
+
+
+@pytest.mark.parametrize('bits', [32, 8])
+def test_groups_and_types_side_by_side(optim, bits):
+    """One norm over every group and type, each group's own hyperparameters; a scheduler moves one of them."""
+    fp32, bf16, fp16 = make([5000, 30], torch.float32), make([4500, 7, 0], torch.bfloat16, 1), make([9000], torch.float16, 2)
+    opt = optim.AdamW([{'params': fp32 + bf16, 'lr': 1e-2}, {'params': fp16, 'lr': 1e-3, 'betas': (0.5, 0.95), 'weight_decay': 0.0}],
+                      max_norm=0.2, state_bits=bits, seed=1)
+    sched = torch.optim.lr_scheduler.LambdaLR(opt, [lambda k: 1.0, lambda k: 0.5 ** k])
+    params = fp32 + bf16 + fp16
+    for k in range(3):
+        before = snapshot(opt, params)
+        opt.step()
+        after = snapshot(opt, params)
+        norm = O.norm([b['g'] for b in before])
+        assert abs(float(opt.total_norm) - norm) <= 3 * O.U * norm
+        # each group against its own formula, under the common factor
+        for lo, hi, hyper in ((0, 5, dict(HYPER, betas=(0.9, 0.999), weight_decay=1e-2)),
+                              (5, 6, dict(lr=1e-3 * 0.5 ** k, betas=(0.5, 0.95), eps=1e-8, weight_decay=0.0))):
+            check_step(params[lo:hi], before[lo:hi], after[lo:hi], hyper, 0.2, 1, opt.total_norm, norm=norm)
+        sched.step()
+
+
+def test_nothing_but_empty_tensors(optim):
+    params = make([0, 0], torch.float32)
+    opt = optim.AdamW(params, max_norm=1.0)
+    opt.step()
+    assert float(opt.total_norm) == 0.0 and float(opt.state[params[0]]['step']) == 1.0
+    assert float(optim.clip_grad_norm_(params, 1.0)) == 0.0
 
 
 @pytest.mark.parametrize('dtype', list(TYPES))
@@ -434,6 +462,10 @@ def test_32bit_checkpoints_are_torchs(optim):
     bad['param_groups'][0]['amsgrad'] = True
     with pytest.raises(ValueError, match='amsgrad'):
         third.load_state_dict(bad)
+    other = torch.optim.RMSprop(b2)
+    other.step()
+    with pytest.raises(ValueError, match='not the state'):
+        third.load_state_dict(other.state_dict())
     with pytest.raises(ValueError, match='groups'):
         optim.AdamW(c[:1], **kw).load_state_dict(sd)
     lr = torch.tensor(7.0, device='cuda')                 # the tensor that a graph reads stays that tensor
