@@ -146,8 +146,6 @@ class ClipRMSprop(torch.optim.Optimizer):
 # ---------------------------------------------------------------------------------------- many tensors at once
 BLOCK = 256                     # elements that share one scale per moment (unetk_adamw_update)
 _CODE, _SCALE = torch.float8_e4m3fn, torch.float8_e8m0fnu
-
-
 _TYPES = {torch.float32, torch.bfloat16, torch.float16}
 
 # one C call per tensor each: a step of small tensors is bound by what the host asks of them
@@ -163,7 +161,9 @@ def _address(words):
 
 def _on_device(device):
     """Launches go to the tensors' device whatever the current one is, on that device's current stream."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    if device.type != 'cuda' or torch.cuda.current_device() == device.index:
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 def _is_dense(t):
@@ -213,8 +213,8 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
         raise ValueError('clip_grad_norm_: a parameter appears twice')
     if len(set(map(_get_device, grads))) != 1:
         raise RuntimeError('clip_grad_norm_: gradients must be on one device')
-    types = set(map(_get_dtype, grads))
-    if not grads[0].is_cuda or not types <= _TYPES or not all(map(_get_contiguous, grads)):
+    types = dict.fromkeys(map(_get_dtype, grads))        # in their order: the norm is summed in it
+    if not grads[0].is_cuda or not types.keys() <= _TYPES or not all(map(_get_contiguous, grads)):
         for g in grads:
             _require(g, 'gradients', 'clip_grad_norm_')
     sets = [(dtype_code(t), grads if len(types) == 1 else [g for g in grads if g.dtype == t]) for t in types]
@@ -428,7 +428,8 @@ class AdamW(torch.optim.Optimizer):
             raise RuntimeError('AdamW.step: no gradients (run backward through the UNet first)')
         plan = self._plan
         pointers = plan.pointers(self) if plan is not None else None
-        with _on_device(next(p.device for g in self.param_groups for p in g['params'])):
+        device = next((p.device for g in self.param_groups for p in g['params']), torch.device('cpu'))
+        with _on_device(device):
             if pointers is None:                         # the first step, or something moved, came or went
                 plan = self._plan = None
                 with torch.no_grad():
@@ -488,6 +489,7 @@ class AdamW(torch.optim.Optimizer):
         # scratch of this call alone, from the allocator of the stream it runs on: calls share none of it
         scratch = torch.empty(plan.words[max_norm is not None], dtype=torch.float64, device=device)
         coefs, partials, norm_ptr, count = scratch.data_ptr(), None, None, 0
+        self.total_norm = None
         if max_norm is not None:
             self.total_norm = torch.empty((), dtype=torch.float32, device=device)
             partials, norm_ptr = coefs + 16 * len(plan.params), self.total_norm.data_ptr()
@@ -546,7 +548,7 @@ class _Plan:
         rows = [r for rs in sets.values() for r in rs]
         self.params, self.absent = [p for p, _, _ in rows], absent
         self.device = rows[0][0].device if rows else None
-        self.counts = [len(g['params']) for g in opt.param_groups]
+        self.every = [list(g['params']) for g in opt.param_groups]
         self.sets, self.tables, first = [], [], 0
         for (at, dtype), rs in sets.items():
             table = array('q', [w for p, st, _ in rs for w in
@@ -559,6 +561,9 @@ class _Plan:
         self.words = [2 * first, 2 * first + sum(int(fn['unetk_grad_partials'](s[3])) for s in self.sets)]
         self.state = list(opt.state.values())
         tensors = list(chain.from_iterable(map(dict.values, self.state)))
+        self.usable = all(map(torch.is_tensor, tensors))      # a user may keep other things there: then every step looks anew
+        if not self.usable:
+            return
         self.refs = list(map(weakref.ref, tensors))
         self.where = list(map(_get_pointer, self.params)) + list(map(_get_pointer, tensors))
         self.types, self.numel = list(map(_get_dtype, self.params)), list(map(_get_numel, self.params))
@@ -569,10 +574,14 @@ class _Plan:
 
     def pointers(self, opt):
         """The gradients' pointers if the plan holds for this step, else None."""
-        params = self.params
+        params, groups = self.params, opt.param_groups
+        if not self.usable or len(groups) != len(self.every):
+            return None
+        for group, had in zip(groups, self.every):
+            if len(group['params']) != len(had) or not all(map(is_, group['params'], had)):
+                return None
         now = list(opt.state.values())
-        if [len(g['params']) for g in opt.param_groups] != self.counts or len(now) != len(self.state) or \
-                not all(map(is_, now, self.state)):
+        if len(now) != len(self.state) or not all(map(is_, now, self.state)):
             return None
         tensors = list(chain.from_iterable(map(dict.values, now)))
         if len(tensors) != len(self.refs) or not all(map(is_, tensors, map(_get_referent, self.refs))) or \

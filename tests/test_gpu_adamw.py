@@ -743,12 +743,20 @@ def test_whatever_moves_between_steps_is_noticed(optim, bits):
         ps.append(make([4500], torch.float32, seed=12)[0])
         o.add_param_group({'params': [ps[-1]], 'lr': 0.5, 'betas': (0.5, 0.6)})
 
+    def other_parameter(o, ps):
+        hold.append(ps[1])
+        ps[1] = make([12], torch.float32, seed=13)[0]
+        o.param_groups[0]['params'][1] = ps[1]
+
+    def a_note(o, ps):
+        o.state[ps[0]]['note'] = 'kept by the user'
+
     def new_rate(o, ps):
         o.param_groups[0]['lr'] *= 3
         o.param_groups[0]['betas'] = (0.5, 0.9)
 
     for change in (None, new_data, None, new_entry, moved_entry, new_state, no_state, no_gradient, None, strided_gradient, new_group,
-                   new_rate, None):
+                   new_rate, other_parameter, a_note, None):
         for i in range(len(params)):
             new = torch.randn(params[i].numel(), generator=g).cuda()
             params[i].grad, twin[i].grad = new, new.clone()
@@ -758,7 +766,11 @@ def test_whatever_moves_between_steps_is_noticed(optim, bits):
         opt.step(), ref.step()
         assert all(torch.equal(p, q) for p, q in zip(params, twin)), change
         assert [float(opt.state[p]['step']) for p in params] == [float(ref.state[q]['step']) for q in twin], change
-    assert float(opt.state[params[3]]['step']) == 15.0 and float(opt.state[params[2]]['step']) == 12.0
+    assert float(opt.state[params[3]]['step']) == 17.0 and float(opt.state[params[2]]['step']) == 14.0
+    for o, ps in ((opt, params), (ref, twin)):
+        ps[0].data = ps[0].data.cpu()
+        with pytest.raises(RuntimeError, match='cuda'):
+            o.step()
 
 
 def test_frozen_parameters_of_a_flat_buffer_stay(optim):
