@@ -376,7 +376,7 @@ int unetk_clip_rmsprop_step(float* param, float* grad, float* square_avg, float*
  * state of zeros.
  *
  * A step is two calls per set of tensors, and every unetk_adamw_prepare of a step comes before its first update:
- * unetk_adamw_prepare: adds 1 to every `step`, writes each tensor's bias corrections to `coefs` (16 bytes a tensor) and, if
+ * unetk_adamw_prepare: adds 1 to every `step`, writes each tensor's bias corrections to `coefs` (16 bytes a tensor, 16-byte aligned) and, if
  *   `partials` is not NULL, sums of squares of the gradients to `partials`.  Returns how many of them it wrote (at most
  *   unetk_grad_partials(n_tensors)) or a negative error.  lr_dev (may be NULL): lr is read from there.
  * unetk_adamw_update: the update; `partials`, `n_partials`: those of ALL sets that the norm covers
