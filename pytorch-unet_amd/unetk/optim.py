@@ -540,8 +540,8 @@ def _all_usual(rows):
 
 
 class _Plan:
-    """What one step found out about its tensors, for the next one: everything but the gradients' pointers, and how to tell that
-    it still holds.  It does not keep the state alive (a user may move that off the device between steps): references tell
+    """The launch tables of an optimizer's own parameters and moments: where they lie, no value of theirs; gradients are looked up
+    at every step.  What one step found out serves the next as long as nothing moved, came or went.  It does not keep the state alive (a user may move that off the device between steps): references tell
     whether a tensor is the same one, its address whether it is where it was."""
 
     def __init__(self, opt, sets, absent):

@@ -1,21 +1,26 @@
 """The many-tensor optimizer step without a GPU: what the entry points refuse, and the 8-bit form's helpers."""
 import ctypes
+import os
 
 import numpy as np
 import pytest
 import torch
 
+from conftest import PKG
 from oracle import adamw_np as O
 
 
 @pytest.fixture(scope='module')
 def nat():
+    if not os.path.exists(os.path.join(PKG, 'libunetk.so')):
+        import __graft_entry__
+        __graft_entry__.build()
     from unetk import _native
     return _native
 
 
 @pytest.fixture(scope='module')
-def optim():
+def optim(nat):
     from unetk import optim
     return optim
 
