@@ -21,13 +21,19 @@ class _UNetImpl:
 
     # ---- forward
     def fwd(self, x):
+        packed = blocks.pack_all(self.net, self.dtype, self.will_backward)   # one launch re-packs every conv weight that changed
+        with blocks.planned(packed):
+            logits, saved = self._fwd_body(x)
+        saved['packed'] = packed
+        return logits, saved
+
+    def _fwd_body(self, x):
         net, dt = self.net, self.dtype
         n, h, w, _, _ = ops.nhwc_meta(x, 'UNet input')
         downs = [net.down1, net.down2, net.down3, net.down4]
         ups = [net.up1, net.up2, net.up3, net.up4]
         enc = [net.inc] + [d.maxpool_conv[1] for d in downs]
         saved = {'enc': [], 'pool_in': [], 'up': [], 'dec': [], 'cats': []}
-        blocks.pack_all(net, dt, self.will_backward)         # one launch re-packs every conv weight that changed
         bn_channels = sum(m.num_features for m in net.modules() if isinstance(m, nn.BatchNorm2d))
         ops.begin_stats_arena(x.device, bn_channels)       # one memset for all BatchNorm statistics of this pass
         # encoder: level k's output is written straight into the first half of that level's concat buffer
@@ -93,7 +99,8 @@ class _UNetImpl:
         # a layer's weight gradient is queued behind the NEXT layer's BatchNorm-backward reduction (blocks.conv_bn_relu_bwd)
         blocks.DEFER_WGRAD = blocks.DEFER_WGRAD_ENABLED
         try:
-            out = self._bwd_body(saved, dlogits, grads, needs, net, ups, enc, done)
+            with blocks.planned(saved['packed']):
+                out = self._bwd_body(saved, dlogits, grads, needs, net, ups, enc, done)
             ops.run_deferred()               # the last layer's
             return out
         finally:

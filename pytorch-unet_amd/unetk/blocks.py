@@ -10,6 +10,7 @@ Reference semantics restated (file:line into the reference):
   up_*            unet/unet_parts.py:49-67   Upsample|ConvTranspose2d -> F.pad -> cat([skip, up])
   head_*          unet/unet_parts.py:74      Conv2d k=1 + bias
 """
+import contextlib
 import os
 
 import torch
@@ -39,14 +40,50 @@ def activation_dtype(x):
     raise RuntimeError(f'unsupported activation dtype {x.dtype}')
 
 
+# (module, kind, dtype) of the packed weights that pack_all has brought up to date for the whole-network pass that runs now
+_PLANNED = frozenset()
+_RECORDED = -1                  # in the place of a version: this packing was recorded into a graph, not done
+
+
+@contextlib.contextmanager
+def planned(packed):
+    """While a whole-network pass runs: packed_weight() takes what pack_all (which returned `packed`) prepared for it."""
+    global _PLANNED
+    prev, _PLANNED = _PLANNED, packed
+    try:
+        yield
+    finally:
+        _PLANNED = prev
+
+
+def wrote_in_place(params):
+    """Kernels wrote `params` behind PyTorch's back: bump their version counters like any in-place op would, so autograd's
+    checks and packed_weight() see it.  A graph that is captured here writes them again at every replay and bumps nothing then:
+    such parameters are marked, and no version is trusted to tell whether a packing of them is current."""
+    torch.autograd.graph.increment_version(params)
+    if torch.cuda.is_current_stream_capturing():
+        for p in params:
+            p._unetk_graph_writes = True
+
+
+def _is_current(hit, w):
+    return (hit is not None and hit[0] == w._version and hit[1] == w.data_ptr()
+            and not getattr(w, '_unetk_graph_writes', False))
+
+
 def packed_weight(mod, kind, dtype, c_out, c_in):
     """Cached MFMA-fragment packing of mod.weight, refreshed when the parameter changes (optimizer step,
-    load_state_dict, .to())."""
+    load_state_dict, .to()), at every pass if a captured graph writes it, and inside every graph that reads it: a replay
+    computes with the weights as they are then."""
     w = mod.weight
     cache = mod.__dict__.setdefault('_unetk_pack', {})
     key = (kind, dtype)
     hit = cache.get(key)
-    if hit is not None and hit[0] == w._version and hit[1] == w.data_ptr():
+    if (mod, kind, dtype) in _PLANNED and hit is not None and hit[0] in (w._version, _RECORDED) and hit[1] == w.data_ptr():
+        return hit[2]
+    if torch.cuda.is_current_stream_capturing():
+        return ops.pack_weight(kind, w, c_out, c_in, dtype)      # the graph's own: nothing eager may take it for done
+    if _is_current(hit, w):
         return hit[2]
     t = ops.pack_weight(kind, w, c_out, c_in, dtype)
     cache[key] = (w._version, w.data_ptr(), t)
@@ -57,7 +94,8 @@ def pack_all(net, dtype, need_dgrad):
     """Refresh the packed weights of EVERY MFMA convolution of `net` in one launch (unetk_pack_plan_*), then let
     packed_weight() hit its cache: 42 per-layer pack launches per training step become one.  The plan (device copy
     of the per-layer records) is cached on the net and rebuilt when a parameter or packed buffer moved; layers whose
-    weights are not plain contiguous fp32 keep the per-layer path."""
+    weights are not plain contiguous fp32 keep the per-layer path, and so do all where a graph is captured before there is a plan
+    (its copy to the device cannot be).  Returns what planned() takes."""
     import ctypes
     import numpy as np
     import torch.nn as nn
@@ -74,20 +112,18 @@ def pack_all(net, dtype, need_dgrad):
             continue
         for kind in kinds if need_dgrad else kinds[:1]:
             targets.append((m, kind, c_out, c_in))
-    if not targets:
-        return
-
-    def stale(t):
-        m, kind = t[0], t[1]
-        hit = m.__dict__.get('_unetk_pack', {}).get((kind, dtype))
-        return hit is None or hit[0] != m.weight._version or hit[1] != m.weight.data_ptr()
-    if not any(stale(t) for t in targets):
-        return
+    capturing = bool(targets) and torch.cuda.is_current_stream_capturing()
+    packed = frozenset((m, kind, dtype) for m, kind, _, _ in targets)
+    if not capturing and all(_is_current(m.__dict__.get('_unetk_pack', {}).get((kind, dtype)), m.weight)
+                             for m, kind, _, _ in targets):
+        return packed
     dc = ops.dtype_code(dtype)
     plans = net.__dict__.setdefault('_unetk_pack_plans', {})
     plan = plans.get((dtype, need_dgrad))
     srcs = tuple(t[0].weight.data_ptr() for t in targets)
     if plan is None or plan['srcs'] != srcs:
+        if capturing:
+            return frozenset()
         es = torch.empty(0, dtype=dtype).element_size()
         bufs = []
         for m, kind, c_out, c_in in targets:
@@ -112,7 +148,9 @@ def pack_all(net, dtype, need_dgrad):
     ops.check(ops.fn['unetk_pack_plan_run'](plan['dev'].data_ptr(), plan['n'], plan['total'], ops.stream_ptr()),
               'unetk_pack_plan_run')
     for (m, kind, _, _), buf in zip(targets, plan['bufs']):
-        m.__dict__.setdefault('_unetk_pack', {})[(kind, dtype)] = (m.weight._version, m.weight.data_ptr(), buf)
+        version = _RECORDED if capturing else m.weight._version
+        m.__dict__.setdefault('_unetk_pack', {})[(kind, dtype)] = (version, m.weight.data_ptr(), buf)
+    return packed
 
 
 def _f32c(p):

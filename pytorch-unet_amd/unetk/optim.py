@@ -21,6 +21,7 @@ import torch
 
 from . import _native as nat
 from ._native import check, dtype_code, fn, stream_ptr
+from .blocks import wrote_in_place
 
 
 class ClipRMSprop(torch.optim.Optimizer):
@@ -135,9 +136,7 @@ class ClipRMSprop(torch.optim.Optimizer):
                                             float(g['lr']), float(g['alpha']), float(g['eps']),
                                             float(g['weight_decay']), float(g['momentum']), stream_ptr()),
               'unetk_clip_rmsprop_step')
-        # the kernel wrote the parameters behind PyTorch's back: bump their version counters like any in-place op
-        # would, so autograd's checks and the packed-weight cache (blocks.packed_weight) see the update
-        torch.autograd.graph.increment_version(self.fg.params)
+        wrote_in_place(self.fg.params)
         self._steps += 1
         self.fg.consume()
         return None
@@ -436,9 +435,7 @@ class AdamW(torch.optim.Optimizer):
                     plan, pointers, copies = self._make_plan()
             if plan.params:
                 self._launch(plan, pointers)
-        if plan.params:
-            # the kernels wrote the parameters behind PyTorch's back: bump their version counters like any in-place op
-            torch.autograd.graph.increment_version(plan.params)
+                wrote_in_place(plan.params)
         self._plan = plan
         if self.fg is not None:
             self.fg.consume()
