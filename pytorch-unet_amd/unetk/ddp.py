@@ -98,8 +98,17 @@ class FlatGrads:
         return dict(self.views)
 
     def consume(self):
-        """The gradients of the last backward pass were applied (optimizer.step) or discarded (zero_grad)."""
+        """The gradients of the last backward pass were applied (optimizer.step)."""
         self._unconsumed = False
+
+    def discard(self, set_to_none=True):
+        """optimizer.zero_grad(): the gradients are gone, as torch's become None -- an optimizer step without a backward pass in
+        between finds none and raises -- or zero with set_to_none=False."""
+        self._unconsumed = False
+        if set_to_none:
+            self.flat, self.views = None, {}
+        elif self.flat is not None:
+            self.flat.zero_()
 
     def bind_param_grads(self):
         """Make every `p.grad` the parameter's view of the flat buffer.  Autograd only *sometimes* keeps the tensor a

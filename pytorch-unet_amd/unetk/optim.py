@@ -36,9 +36,10 @@ class ClipRMSprop(torch.optim.Optimizer):
 
     def zero_grad(self, set_to_none=True):
         """train.py:113.  The flat gradient buffer is rewritten by every backward pass, so there is nothing to zero;
-        the call marks the previous pass's gradients as discarded (a backward without it or step() in between would be
-        gradient accumulation, which the flat buffer does not do: FlatGrads.initial_grads raises)."""
-        self.fg.consume()
+        the call discards the previous pass's gradients, so that a step() before the next pass does not apply them again (a
+        backward without it or step() in between would be gradient accumulation, which the flat buffer does not do:
+        FlatGrads.initial_grads raises)."""
+        self.fg.discard(set_to_none)
         super().zero_grad(set_to_none=set_to_none)
 
     # ---- checkpoint / resume in torch.optim.RMSprop's own format (train.py saves only the model's state_dict, but a
@@ -346,7 +347,7 @@ class AdamW(torch.optim.Optimizer):
 
     def zero_grad(self, set_to_none=True):
         if self.fg is not None:
-            self.fg.consume()
+            self.fg.discard(set_to_none)
         super().zero_grad(set_to_none=set_to_none)
 
     # ---- state

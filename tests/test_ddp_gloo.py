@@ -132,3 +132,23 @@ def test_bucket_schedule_of_the_reference_unet():
         dist.all_reduce = orig
     assert sum(calls) == sync2.total and max(calls) * 4 <= 30 << 20 and calls[-1] * 4 <= 2 << 20
     assert [b - a for a, b in sync2.launched] == calls
+
+
+def test_discarded_gradients_are_gone():
+    from unet import UNet
+    from unetk.ddp import FlatGrads
+    net = UNet(3, 2, True)
+    sync = FlatGrads(net)
+    first = sync.initial_grads()
+    sync.flat.fill_(1.0)
+    sync.discard(set_to_none=False)
+    assert not sync.flat.any() and all(not g.any() for g in first.values())
+    sync.initial_grads()                                     # no accumulation
+    sync.consume()
+    assert sync.flat is not None                             # applied gradients may be applied again
+    sync.discard()
+    assert sync.flat is None and sync.views == {}
+    sync.bind_param_grads()
+    assert all(p.grad is None for p in net.parameters())
+    sync.finish()
+    assert len(sync.initial_grads()) == len(sync.params)

@@ -132,3 +132,35 @@ def test_a_forward_captured_before_any_other(optim):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize('kind', ['adamw', 'rmsprop'])
+def test_discarded_gradients_of_a_flat_buffer_are_not_applied_again(optim, kind):
+    from unetk.ddp import FlatGrads
+    net = make_net()
+    fg = FlatGrads(net, grads_to_autograd=False)
+    kw = dict(lr=1e-2, weight_decay=0.1)
+    opt = optim.AdamW(fg, **kw) if kind == 'adamw' else optim.ClipRMSprop(fg, max_norm=1.0, **kw)
+    for _ in range(2):
+        fg.initial_grads()
+        fg.flat.normal_()
+        opt.step()
+        opt.step()                                     # the same gradients again, as a stock optimizer would
+        kept = [p.detach().clone() for p in net.parameters()]
+        opt.zero_grad()
+        with pytest.raises(RuntimeError, match='no gradients'):
+            opt.step()
+        assert all(torch.equal(p, q) for p, q in zip(net.parameters(), kept))
+    if kind == 'adamw':
+        assert float(opt.state[net.outc.conv.weight]['step']) == 4.0
+    # gradients of zero are gradients: the decay goes on, the next backward pass is no accumulation
+    fg.initial_grads()
+    fg.flat.normal_()
+    opt.zero_grad(set_to_none=False)
+    assert not fg.flat.any() and not any(v.any() for v in fg.views.values())
+    opt.step()
+    assert not any(torch.equal(p, q) for p, q in zip(net.parameters(), kept) if q.any())
+    opt.zero_grad(set_to_none=False)
+    fg.initial_grads()
+    with pytest.raises(RuntimeError, match='accumulation'):
+        fg.initial_grads()
