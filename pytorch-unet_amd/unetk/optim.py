@@ -229,8 +229,11 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
             count += _written(fn['unetk_grad_sumsq'](_address(pointers), _address(numel), n, code, at + 8 * count, stream),
                               'unetk_grad_sumsq')
         if error_if_nonfinite:
-            total = partials[:count].sum().sqrt()
-            if not bool(torch.isfinite(total)):
+            # the very norm that is returned and divided by (fp32: infinite where the sum in fp64 is not), before anything is scaled
+            zero = array('q', [0])
+            check(fn['unetk_grad_clip'](_address(zero), _address(zero), 1, sets[0][0], at, count, max_norm, norm.data_ptr(), stream),
+                  'unetk_grad_clip')
+            if not bool(torch.isfinite(norm)):
                 raise RuntimeError('clip_grad_norm_: the norm of the gradients is not finite, so they cannot be clipped')
         for code, n, pointers, numel in sets:
             check(fn['unetk_grad_clip'](_address(pointers), _address(numel), n, code, at, count, max_norm, norm.data_ptr(),

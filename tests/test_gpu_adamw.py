@@ -612,6 +612,23 @@ def test_clip_of_huge_and_tiny_gradients(optim):
         assert abs(got - want) <= 3 * O.U * want
 
 
+def test_a_norm_beyond_fp32_is_not_finite(optim):
+    """A thousand times 1e38: the sum of squares is finite in fp64, the fp32 norm that divides the gradients is not."""
+    for dtype in (torch.float32, torch.bfloat16):
+        p = [torch.nn.Parameter(torch.zeros(n, dtype=dtype, device='cuda')) for n in (1000, 7)]
+        for q in p:
+            q.grad = torch.full_like(q, 1e38)
+        kept = [q.grad.clone() for q in p]
+        with pytest.raises(RuntimeError, match='not finite'):
+            optim.clip_grad_norm_(p, 1.0, error_if_nonfinite=True)
+        assert all(torch.equal(q.grad, k) for q, k in zip(p, kept))
+        for q in p:
+            q.grad.fill_(1e37)
+        got = float(optim.clip_grad_norm_(p, 1.0, error_if_nonfinite=True))
+        want = float(p[0].detach().new_tensor(1e37)) * math.sqrt(1007)
+        assert abs(got - want) <= 3 * O.U * want
+
+
 def test_more_than_two_to_the_31_elements(optim):
     """Offsets beyond 32 bits: the last elements of a tensor of 2^31 + 4099."""
     n, tail = 2 ** 31 + 4099, 5000
