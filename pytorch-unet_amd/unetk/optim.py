@@ -480,7 +480,13 @@ class AdamW(torch.optim.Optimizer):
 
     def _launch(self, plan, pointers):
         stream, device = stream_ptr(), plan.device
+        # all that can be wrong with the groups is found here: once a launch has counted, the step has to go through
+        hyper = [_hyperparameters(self.param_groups[at], device) for at, _, _, _, _ in plan.sets]
         max_norm = self.param_groups[0]['max_norm']
+        if max_norm is not None:
+            max_norm = float(max_norm)
+            if not max_norm > 0:
+                raise ValueError(f'AdamW: max_norm must be positive or None, got {max_norm}')
         grad_scale, found_inf = getattr(self, 'grad_scale', None), getattr(self, 'found_inf', None)
         for t in (grad_scale, found_inf):
             if t is not None and (t.dtype != torch.float32 or t.device != device or t.numel() != 1):
@@ -495,25 +501,26 @@ class AdamW(torch.optim.Optimizer):
             self.total_norm = torch.empty((), dtype=torch.float32, device=device)
             partials, norm_ptr = coefs + 16 * len(plan.params), self.total_norm.data_ptr()
         grads = _address(pointers)
-        for at, code, first, n, table in plan.sets:
-            group = self.param_groups[at]
-            lr, lr_ptr = group['lr'], None
-            if isinstance(lr, torch.Tensor):
-                if lr.is_cuda:
-                    if lr.dtype != torch.float32 or lr.device != device or lr.numel() != 1:
-                        raise RuntimeError("AdamW: a tensor lr must be an fp32 scalar on the parameters' device")
-                    lr, lr_ptr = 0.0, lr.data_ptr()
-                else:
-                    lr = float(lr)
-            count += _written(fn['unetk_adamw_prepare'](table, grads + 8 * first, n, code, lr, lr_ptr, *group['betas'],
-                                                        group['weight_decay'], self.seed, found_ptr, coefs + 16 * first,
+        for (_, code, first, n, table), (lr, lr_ptr, beta1, beta2, _, weight_decay) in zip(plan.sets, hyper):
+            count += _written(fn['unetk_adamw_prepare'](table, grads + 8 * first, n, code, lr, lr_ptr, beta1, beta2, weight_decay,
+                                                        self.seed, found_ptr, coefs + 16 * first,
                                                         partials + 8 * count if partials else None, stream),
                               'unetk_adamw_prepare')
-        for at, code, first, n, table in plan.sets:
-            group = self.param_groups[at]
-            check(fn['unetk_adamw_update'](table, grads + 8 * first, n, code, *group['betas'], group['eps'], scale_ptr, found_ptr,
+        for (_, code, first, n, table), (_, _, beta1, beta2, eps, _) in zip(plan.sets, hyper):
+            check(fn['unetk_adamw_update'](table, grads + 8 * first, n, code, beta1, beta2, eps, scale_ptr, found_ptr,
                                            coefs + 16 * first, partials, count, max_norm or 0.0, norm_ptr, stream),
                   'unetk_adamw_update')
+
+
+def _hyperparameters(group, device):
+    """(lr, pointer to an lr on the device or None, beta1, beta2, eps, weight_decay) as a launch takes them."""
+    lr, lr_ptr = group['lr'], None
+    if isinstance(lr, torch.Tensor) and lr.is_cuda:
+        if lr.dtype != torch.float32 or lr.device != device or lr.numel() != 1:
+            raise RuntimeError("AdamW: a tensor lr must be an fp32 scalar on the parameters' device")
+        lr, lr_ptr = 0.0, lr.data_ptr()
+    beta1, beta2 = group['betas']
+    return float(lr), lr_ptr, float(beta1), float(beta2), float(group['eps']), float(group['weight_decay'])
 
 
 def _all_usual(rows):

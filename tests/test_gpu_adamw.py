@@ -580,6 +580,30 @@ def test_refusals(optim):
         opt.step()
 
 
+@pytest.mark.parametrize('key,value,error', [
+    ('lr', torch.tensor(1e-3, dtype=torch.float64), None), ('lr', 'fast', ValueError), ('betas', (0.9,), ValueError),
+    ('betas', (0.9, None), TypeError), ('eps', None, TypeError), ('weight_decay', 'none', ValueError), ('max_norm', -1.0, ValueError),
+    ('max_norm', float('nan'), ValueError), ('max_norm', 0.0, ValueError)])
+def test_a_step_that_fails_has_not_counted(optim, key, value, error):
+    """What is wrong with the last group is found before the first group's launch."""
+    a, b = make([5000, 3], torch.float32), make([40], torch.float32, 1)
+    opt = optim.AdamW([{'params': a}, {'params': b}], **HYPER, max_norm=0.5)
+    opt.step()
+    good = opt.param_groups[1][key]
+    before = snapshot(opt, a + b)
+    for g in opt.param_groups[0 if key == 'max_norm' else 1:]:
+        g[key] = value.cuda() if torch.is_tensor(value) else value
+    with pytest.raises(error or RuntimeError):
+        opt.step()
+    after = snapshot(opt, a + b)
+    for x, y in zip(before, after):
+        assert x['t'] == y['t'] == 1.0 and all(np.array_equal(x[k], y[k]) for k in 'pmv')
+    for g in opt.param_groups:
+        g[key] = good
+    opt.step()
+    check_step(a + b, before, snapshot(opt, a + b), HYPER, 0.5, 0, opt.total_norm)
+
+
 # ------------------------------------------------------------------------------------------------------------- clip
 @pytest.mark.parametrize('sizes', list(SIZES))
 @pytest.mark.parametrize('dtype', list(TYPES) + ['mixed'])
