@@ -329,10 +329,7 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError(f'AdamW: {k} must not be negative, got {g[k]}')
         if not all(0.0 <= b < 1.0 for b in g['betas']):
             raise ValueError(f"AdamW: betas must lie in [0, 1), got {g['betas']}")
-        if g['max_norm'] is not None and not g['max_norm'] > 0:
-            raise ValueError(f"AdamW: max_norm must be positive or None, got {g['max_norm']}")
-        if g['max_norm'] != self.param_groups[0]['max_norm']:
-            raise ValueError('AdamW: the clip is over all groups: max_norm must be the same in each')
+        _common_max_norm([g, self.param_groups[0]])
         if self.fg is not None and not all(id(p) in self.fg.offsets for p in g['params']):
             raise ValueError('AdamW: a parameter has no place in the flat gradient buffer')
         for p in g['params']:
@@ -482,11 +479,7 @@ class AdamW(torch.optim.Optimizer):
         stream, device = stream_ptr(), plan.device
         # all that can be wrong with the groups is found here: once a launch has counted, the step has to go through
         hyper = [_hyperparameters(self.param_groups[at], device) for at, _, _, _, _ in plan.sets]
-        max_norm = self.param_groups[0]['max_norm']
-        if max_norm is not None:
-            max_norm = float(max_norm)
-            if not max_norm > 0:
-                raise ValueError(f'AdamW: max_norm must be positive or None, got {max_norm}')
+        max_norm = _common_max_norm(self.param_groups)
         grad_scale, found_inf = getattr(self, 'grad_scale', None), getattr(self, 'found_inf', None)
         for t in (grad_scale, found_inf):
             if t is not None and (t.dtype != torch.float32 or t.device != device or t.numel() != 1):
@@ -510,6 +503,18 @@ class AdamW(torch.optim.Optimizer):
             check(fn['unetk_adamw_update'](table, grads + 8 * first, n, code, beta1, beta2, eps, scale_ptr, found_ptr,
                                            coefs + 16 * first, partials, count, max_norm or 0.0, norm_ptr, stream),
                   'unetk_adamw_update')
+
+
+def _common_max_norm(groups):
+    """The one limit of all groups, as a float or None."""
+    max_norm = groups[0]['max_norm']
+    if max_norm is not None:
+        max_norm = float(max_norm)
+        if not max_norm > 0:
+            raise ValueError(f'AdamW: max_norm must be positive or None, got {max_norm}')
+    if any(g['max_norm'] != max_norm for g in groups):
+        raise ValueError('AdamW: the clip is over all groups: max_norm must be the same in each')
+    return max_norm
 
 
 def _hyperparameters(group, device):

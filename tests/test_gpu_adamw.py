@@ -604,6 +604,22 @@ def test_a_step_that_fails_has_not_counted(optim, key, value, error):
     check_step(a + b, before, snapshot(opt, a + b), HYPER, 0.5, 0, opt.total_norm)
 
 
+def test_a_limit_of_one_group_alone_is_refused_at_the_step(optim):
+    a, b = make([5000, 3], torch.float32), make([40], torch.float32, 1)
+    opt = optim.AdamW([{'params': a}, {'params': b}], **HYPER)
+    for first, second in ((None, 0.5), (0.5, None), (0.5, 0.25)):
+        opt.param_groups[0]['max_norm'], opt.param_groups[1]['max_norm'] = first, second
+        before = snapshot(opt, a + b)
+        with pytest.raises(ValueError, match='same in each'):
+            opt.step()
+        assert all(x['t'] == y['t'] and np.array_equal(x['p'], y['p']) for x, y in zip(before, snapshot(opt, a + b)))
+    for g in opt.param_groups:                                        # in both it is the clip, as from the start
+        g['max_norm'] = 0.25
+    before = snapshot(opt, a + b)
+    opt.step()
+    check_step(a + b, before, snapshot(opt, a + b), HYPER, 0.25, 0, opt.total_norm)
+
+
 # ------------------------------------------------------------------------------------------------------------- clip
 @pytest.mark.parametrize('sizes', list(SIZES))
 @pytest.mark.parametrize('dtype', list(TYPES) + ['mixed'])
