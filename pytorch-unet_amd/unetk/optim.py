@@ -12,6 +12,7 @@ buffer of unetk.ddp.FlatGrads, the optimizer state is two more flat buffers, and
 (or the flat buffers above), decoupled weight decay, moments in 32 or in 8 bits, the clip in front of the step or by itself.
 """
 import contextlib
+import copy
 import weakref
 from array import array
 from itertools import chain
@@ -324,18 +325,22 @@ class AdamW(torch.optim.Optimizer):
     def _check_group(self, g):
         if len({id(p) for p in g['params']}) != len(g['params']):
             raise ValueError('AdamW: a parameter appears twice')
-        for k in ('lr', 'eps', 'weight_decay'):
-            if not isinstance(g[k], torch.Tensor) and not g[k] >= 0:
-                raise ValueError(f'AdamW: {k} must not be negative, got {g[k]}')
-        if not all(0.0 <= b < 1.0 for b in g['betas']):
-            raise ValueError(f"AdamW: betas must lie in [0, 1), got {g['betas']}")
-        _common_max_norm([g, self.param_groups[0]])
+        self._check_hyperparameters(g, [g, self.param_groups[0]])
         if self.fg is not None and not all(id(p) in self.fg.offsets for p in g['params']):
             raise ValueError('AdamW: a parameter has no place in the flat gradient buffer')
         for p in g['params']:
             _require(p, 'parameters')
             if p.device != next(q for h in self.param_groups for q in h['params']).device:
                 raise RuntimeError('AdamW: parameters must be on one device')
+
+    @staticmethod
+    def _check_hyperparameters(g, groups):
+        for k in ('lr', 'eps', 'weight_decay'):
+            if not isinstance(g[k], torch.Tensor) and not g[k] >= 0:
+                raise ValueError(f'AdamW: {k} must not be negative, got {g[k]}')
+        if not all(0.0 <= b < 1.0 for b in g['betas']):
+            raise ValueError(f"AdamW: betas must lie in [0, 1), got {g['betas']}")
+        _common_max_norm(groups)
 
     def __getstate__(self):
         return {**super().__getstate__(), 'fg': self.fg, 'state_bits': self.state_bits, 'min_8bit_numel': self.min_8bit_numel,
@@ -406,14 +411,15 @@ class AdamW(torch.optim.Optimizer):
             bits = 8 if self.state_bits == 8 and p.numel() >= self.min_8bit_numel else 32
             state[p] = _fit_moments(p, st, bits)
             state[p]['step'] = torch.tensor(float(st['step']), dtype=torch.float32, device=p.device)
-        for own, g in zip(self.param_groups, groups):
-            for k in ('betas', 'eps', 'weight_decay', 'max_norm', 'initial_lr'):
-                if k in g:
-                    own[k] = g[k]
+        # a group takes over all that the file's holds (a scheduler's entries too) and keeps what the file's lacks
+        merged = [{**own, **{k: copy.deepcopy(v) for k, v in g.items() if k != 'params'}, 'lr': float(g['lr'])}
+                  for own, g in zip(self.param_groups, groups)]
+        for g in merged:
+            self._check_hyperparameters(g, merged)
+        for own, g in zip(self.param_groups, merged):
             if isinstance(own['lr'], torch.Tensor):      # a captured graph reads this very tensor
-                own['lr'].fill_(float(g['lr']))
-            else:
-                own['lr'] = float(g['lr'])
+                g['lr'] = own['lr'].fill_(g['lr'])
+            own.update(g)
         self._plan = None
         self.state.clear()
         self.state.update(state)

@@ -504,6 +504,47 @@ def test_8bit_checkpoints_resume_to_the_bit_and_convert(optim, tmp_path):
         assert torch.equal(oa.state[a[1]][k].view(torch.uint8), ob.state[b[1]][k].view(torch.uint8))
 
 
+def test_a_loaded_group_keeps_what_its_scheduler_put_there(optim):
+    """Resuming a one-cycle run: the group's entries come back from either class's file, and the runs go on together."""
+    sched = torch.optim.lr_scheduler.OneCycleLR
+
+    def run(cls, params, steps, opt=None, file=None):
+        opt = cls(params, lr=1e-3, betas=(0.9, 0.99))
+        if file is not None:
+            opt.load_state_dict(file['opt'])
+        s = sched(opt, max_lr=1e-2, total_steps=20, last_epoch=-1 if file is None else 3)
+        if file is not None:
+            s.load_state_dict(file['sched'])
+        rates = []
+        for k in range(steps):
+            for p in params:
+                p.grad = torch.full_like(p, 0.1 + k)
+            opt.step(), s.step()
+            rates.append((opt.param_groups[0]['lr'], opt.param_groups[0]['betas'][0]))
+        return rates, dict(opt=copy.deepcopy(opt.state_dict()), sched=s.state_dict()), opt
+
+    want, _, _ = run(torch.optim.AdamW, make([300], torch.float32), 9)
+    for first in (optim.AdamW, torch.optim.AdamW):
+        for second in (optim.AdamW, torch.optim.AdamW):
+            a, file, _ = run(first, make([300], torch.float32), 4)
+            b, _, opt = run(second, make([300], torch.float32), 5, file=file)
+            assert np.allclose(a + b, want, rtol=1e-12)
+            assert opt.param_groups[0]['max_lr'] == 1e-2 and opt.param_groups[0]['initial_lr'] == file['opt']['param_groups'][0]['initial_lr']
+    # what the file lacks stays (torch's knows no max_norm); what it holds is a copy and has to be sound
+    opt = optim.AdamW(make([300], torch.float32), max_norm=0.5)
+    _, file, _ = run(torch.optim.AdamW, make([300], torch.float32), 1)
+    file['opt']['param_groups'][0]['notes'] = [1]
+    opt.load_state_dict(file['opt'])
+    file['opt']['param_groups'][0]['notes'].append(2)
+    assert opt.param_groups[0]['max_norm'] == 0.5 and opt.param_groups[0]['notes'] == [1]
+    for key, value in (('betas', (1.0, 0.9)), ('eps', -1.0), ('max_norm', 0.0)):
+        bad = copy.deepcopy(file['opt'])
+        bad['param_groups'][0].update({key: value, 'lr': 7.0})
+        with pytest.raises(ValueError, match=key):
+            opt.load_state_dict(bad)
+        assert opt.param_groups[0]['lr'] != 7.0
+
+
 def test_copies_of_the_optimizer_and_a_state_that_leaves_the_device(optim):
     a = make([300, 70001], torch.float32)
     oa = optim.AdamW(a, **HYPER, state_bits=8, seed=3, max_norm=0.5)
