@@ -392,6 +392,10 @@ class AdamW(torch.optim.Optimizer):
 
     # ---- checkpoint / resume.  The file's form (32-bit as torch.optim.AdamW writes it, or 8-bit) need not be this one's.
     def load_state_dict(self, state_dict):
+        state_dict = dict(state_dict)                    # a hook may exchange entries
+        for hook in list(self._optimizer_load_state_dict_pre_hooks.values()):
+            changed = hook(self, state_dict)
+            state_dict = state_dict if changed is None else changed
         groups = state_dict['param_groups']
         if [len(g['params']) for g in groups] != [len(g['params']) for g in self.param_groups]:
             raise ValueError('AdamW.load_state_dict: expected the same parameter groups')
@@ -423,6 +427,8 @@ class AdamW(torch.optim.Optimizer):
         self._plan = None
         self.state.clear()
         self.state.update(state)
+        for hook in list(self._optimizer_load_state_dict_post_hooks.values()):
+            hook(self)
 
     # ---- step
     def step(self, closure=None):

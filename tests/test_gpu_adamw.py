@@ -545,6 +545,35 @@ def test_a_loaded_group_keeps_what_its_scheduler_put_there(optim):
         assert opt.param_groups[0]['lr'] != 7.0
 
 
+@pytest.mark.parametrize('ours', [True, False])
+def test_load_state_dict_calls_its_hooks(optim, ours):
+    """As torch.optim.AdamW does: pre-hooks in turn, each on what the one before returned, then the load, then the others."""
+    cls, seen = (optim if ours else torch.optim).AdamW, []
+    opt = cls(make([300], torch.float32), lr=1e-3)
+    opt.step()
+    file = opt.state_dict()
+
+    def change(o, sd):
+        seen.append(('change', sd['param_groups'][0]['lr']))
+        return {**sd, 'param_groups': [{**sd['param_groups'][0], 'lr': 0.5}]}
+
+    def look(o, sd):
+        seen.append(('look', sd['param_groups'][0]['lr']))
+        sd['note'] = 1
+
+    opt.register_load_state_dict_pre_hook(change)
+    opt.register_load_state_dict_pre_hook(look)
+    gone = opt.register_load_state_dict_pre_hook(lambda o, sd: seen.append('gone'))
+    first = opt.register_load_state_dict_pre_hook(look, prepend=True)
+    opt.register_load_state_dict_post_hook(lambda o: seen.append(('post', o.param_groups[0]['lr'])))
+    gone.remove()
+    opt.load_state_dict(file)
+    assert seen == [('look', 1e-3), ('change', 1e-3), ('look', 0.5), ('post', 0.5)]
+    assert file['param_groups'][0]['lr'] == 1e-3 and 'note' not in file and opt.param_groups[0]['lr'] == 0.5
+    first.remove()
+    copy.deepcopy(opt).load_state_dict(file)
+
+
 def test_copies_of_the_optimizer_and_a_state_that_leaves_the_device(optim):
     a = make([300, 70001], torch.float32)
     oa = optim.AdamW(a, **HYPER, state_bits=8, seed=3, max_norm=0.5)
