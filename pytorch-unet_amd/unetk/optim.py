@@ -408,10 +408,15 @@ class AdamW(torch.optim.Optimizer):
             if index not in state_dict['state']:
                 continue
             st = state_dict['state'][index]
-            if 'step' not in st or 'exp_avg' not in st or not ('exp_avg_sq' in st or {'exp_avg_root', 'scales'} <= set(st)):
+            if not {'step', 'exp_avg', *(('exp_avg_root',) if 'scales' in st else ('exp_avg_sq',))} <= set(st):
                 raise ValueError('AdamW.load_state_dict: not the state of an AdamW')
-            if tuple(st['exp_avg'].shape) != tuple(p.shape):
+            second = 'exp_avg_root' if 'scales' in st else 'exp_avg_sq'
+            if any(tuple(st[k].shape) != tuple(p.shape) for k in ('exp_avg', second)):
                 raise ValueError('AdamW.load_state_dict: state shape does not match the parameter')
+            if 'scales' in st and (any(st[k].dtype != _CODE for k in ('exp_avg', second)) or st['scales'].dtype != _SCALE
+                                   or tuple(st['scales'].shape) != (-(-p.numel() // BLOCK), 2)):
+                raise ValueError('AdamW.load_state_dict: 8-bit moments must be float8_e4m3fn with float8_e8m0fnu scales of shape '
+                                 '[ceil(numel / 256), 2]')
             bits = 8 if self.state_bits == 8 and p.numel() >= self.min_8bit_numel else 32
             state[p] = _fit_moments(p, st, bits)
             state[p]['step'] = torch.tensor(float(st['step']), dtype=torch.float32, device=p.device)

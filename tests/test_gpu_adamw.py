@@ -574,6 +574,35 @@ def test_load_state_dict_calls_its_hooks(optim, ours):
     copy.deepcopy(opt).load_state_dict(file)
 
 
+@pytest.mark.parametrize('bits', [32, 8])
+def test_a_file_whose_moments_do_not_fit_is_refused(optim, bits):
+    """Neither spread over the parameter nor read as something else: every moment has the parameter's shape, codes are codes."""
+    opt = optim.AdamW(make([300, 5000], torch.float32), state_bits=bits)
+    opt.step()
+    file = opt.state_dict()
+    one = torch.ones(1, device='cuda')
+    changes = [('exp_avg_sq', one), ('exp_avg_sq', torch.zeros((), device='cuda')), ('exp_avg', one)] if bits == 32 else [
+        ('exp_avg', one.to(torch.float8_e4m3fn)), ('exp_avg_root', one.to(torch.float8_e4m3fn)), ('exp_avg_root', None),
+        ('exp_avg', torch.zeros(5000, device='cuda')), ('exp_avg_root', torch.zeros(5000, dtype=torch.uint8, device='cuda')),
+        ('scales', file['state'][1]['scales'][:1]), ('scales', file['state'][1]['scales'].view(torch.uint8)),
+        ('scales', file['state'][1]['scales'][:, :1])]
+    for target in (32, 8):
+        other = optim.AdamW(make([300, 5000], torch.float32, 1), state_bits=target)
+        other.step()
+        params = other.param_groups[0]['params']
+        before = snapshot(other, params)
+        for key, value in changes:
+            bad = copy.deepcopy(file)
+            bad['state'][1][key] = value
+            if value is None:
+                del bad['state'][1][key]
+            with pytest.raises(ValueError, match='load_state_dict'):
+                other.load_state_dict(bad)
+        for x, y in zip(before, snapshot(other, params)):
+            assert x['t'] == y['t'] and np.array_equal(x['m'], y['m']) and np.array_equal(x['v'], y['v'])
+        other.load_state_dict(file)
+
+
 def test_copies_of_the_optimizer_and_a_state_that_leaves_the_device(optim):
     a = make([300, 70001], torch.float32)
     oa = optim.AdamW(a, **HYPER, state_bits=8, seed=3, max_norm=0.5)
