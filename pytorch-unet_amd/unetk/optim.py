@@ -571,8 +571,9 @@ def _all_usual(rows):
 
 class _Plan:
     """The launch tables of an optimizer's own parameters and moments: where they lie, no value of theirs; gradients are looked up
-    at every step.  What one step found out serves the next as long as nothing moved, came or went.  It does not keep the state alive (a user may move that off the device between steps): references tell
-    whether a tensor is the same one, its address whether it is where it was."""
+    at every step.  What one step found out serves the next as long as nothing moved, came or went.  It does not keep the state
+    alive, neither its tensors nor the dictionaries that hold them (a user may move it off the device or drop it between steps):
+    weak references tell whether a tensor is the same one, its address whether it is where it was."""
 
     def __init__(self, opt, sets, absent):
         rows = [r for rs in sets.values() for r in rs]
@@ -589,8 +590,8 @@ class _Plan:
             self.sets.append((at, dtype_code(dtype), first, len(rs), _address(table)))
             first += len(rs)
         self.words = [2 * first, 2 * first + sum(int(fn['unetk_grad_partials'](s[3])) for s in self.sets)]
-        self.state = list(opt.state.values())
-        tensors = list(chain.from_iterable(map(dict.values, self.state)))
+        self.owners = list(opt.state)
+        tensors = list(chain.from_iterable(map(dict.values, opt.state.values())))
         self.usable = all(map(torch.is_tensor, tensors))      # a user may keep other things there: then every step looks anew
         if not self.usable:
             return
@@ -610,10 +611,9 @@ class _Plan:
         for group, had in zip(groups, self.every):
             if len(group['params']) != len(had) or not all(map(is_, group['params'], had)):
                 return None
-        now = list(opt.state.values())
-        if len(now) != len(self.state) or not all(map(is_, now, self.state)):
+        if len(opt.state) != len(self.owners) or not all(map(is_, opt.state, self.owners)):
             return None
-        tensors = list(chain.from_iterable(map(dict.values, now)))
+        tensors = list(chain.from_iterable(map(dict.values, opt.state.values())))
         if len(tensors) != len(self.refs) or not all(map(is_, tensors, map(_get_referent, self.refs))) or \
                 list(map(_get_pointer, params)) + list(map(_get_pointer, tensors)) != self.where:
             return None

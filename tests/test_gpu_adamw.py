@@ -629,6 +629,41 @@ def test_copies_of_the_optimizer_and_a_state_that_leaves_the_device(optim):
         assert torch.equal(p, q) and torch.equal(p, r)
 
 
+@pytest.mark.parametrize('bits', [32, 8])
+def test_a_state_that_is_dropped_or_replaced_frees_its_memory(optim, bits):
+    """The step's own bookkeeping holds neither the tensors nor the dictionaries they are in."""
+    n = 1 << 22
+    opt = optim.AdamW(make([n, 300], torch.float32), state_bits=bits)
+    p = opt.param_groups[0]['params'][0]
+
+    def freed(change):
+        opt.step(), opt.step()
+        held = torch.cuda.memory_allocated()
+        change()
+        return held - torch.cuda.memory_allocated()
+
+    def off():
+        opt.state[p] = {k: v.cpu() for k, v in opt.state[p].items()}
+
+    at_least = n * 8 if bits == 32 else n * 2
+    assert freed(off) >= at_least
+    with pytest.raises(RuntimeError, match='state'):
+        opt.step()
+    opt.state[p] = {k: v.cuda() for k, v in opt.state[p].items()}
+    assert freed(lambda: opt.state.pop(p)) >= at_least
+    assert freed(opt.state.clear) >= at_least
+    opt.step()
+    assert float(opt.state[p]['step']) == 1.0
+    # two parameters that exchange their states: each goes on with the other's moments, as the dictionary says
+    a, b = make([400, 400], torch.float32)
+    opt = optim.AdamW([a, b], **HYPER, state_bits=bits, min_8bit_numel=1)
+    opt.step(), opt.step()
+    opt.state[a], opt.state[b] = opt.state[b], opt.state[a]
+    before = snapshot(opt, [a, b])
+    opt.step()
+    check_step([a, b], before, snapshot(opt, [a, b]), HYPER)
+
+
 @pytest.mark.skipif(torch.cuda.device_count() < 2, reason='one GPU')
 def test_parameters_on_another_device_than_the_current_one(optim):
     p = make([5000, 40], torch.float32)
