@@ -284,7 +284,8 @@ class AdamW(torch.optim.Optimizer):
     flat gradient buffer is then read in place.  Any dense memory layout; a gradient that is laid out unlike its parameter is
     copied first.
     max_norm: limit of the 2-norm of all gradients together (one value for all groups), None for no clip.  The gradients
-    themselves stay as they are; `total_norm` holds the norm before the clip (fp32, on the device) after a step.
+    themselves stay as they are; `total_norm` holds the norm before the clip (fp32, on the device) after a step, zero if there
+    were none.
     state_bits: 32 keeps `exp_avg` and `exp_avg_sq` in fp32 whatever the parameter's type.  8 keeps them as fp8 codes with a
     power-of-two scale per 256 elements (2.02 instead of 8 bytes a parameter), rounded stochastically from `seed`, the step and the
     element's index, for tensors of at least `min_8bit_numel` elements; smaller ones (biases, BatchNorm) keep 32 bits.
@@ -454,6 +455,9 @@ class AdamW(torch.optim.Optimizer):
             if plan.params:
                 self._launch(plan, pointers)
                 wrote_in_place(plan.params)
+            else:                                        # no gradients: a norm of zero, not an earlier step's
+                limit = _common_max_norm(self.param_groups)
+                self.total_norm = None if limit is None else torch.zeros((), dtype=torch.float32, device=device)
         self._plan = plan
         if self.fg is not None:
             self.fg.consume()

@@ -162,6 +162,19 @@ def test_nothing_but_empty_tensors(optim):
     assert float(optim.clip_grad_norm_(params, 1.0)) == 0.0
 
 
+def test_the_norm_of_no_gradients_is_zero(optim):
+    params = make([50, 5000], torch.float32)
+    opt = optim.AdamW(params, max_norm=1.0)
+    opt.step()
+    assert float(opt.total_norm) > 0
+    opt.zero_grad()
+    opt.step()
+    assert opt.total_norm.is_cuda and opt.total_norm.dtype == torch.float32 and float(opt.total_norm) == 0.0
+    opt.param_groups[0]['max_norm'] = None
+    opt.step()
+    assert opt.total_norm is None
+
+
 @pytest.mark.parametrize('dtype', list(TYPES))
 @pytest.mark.parametrize('bits', [32, 8])
 @pytest.mark.parametrize('shift', [1, 3])
