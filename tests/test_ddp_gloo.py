@@ -1,6 +1,8 @@
 """Data-parallel gradient bucketing (unetk/ddp.py) with world_size 2 on CPU/gloo: the flat buffer is laid out in
 backward-completion order, buckets fire as layers complete, and every rank ends with the average."""
+import copy
 import os
+import pickle
 import socket
 
 import pytest
@@ -152,3 +154,39 @@ def test_discarded_gradients_are_gone():
     assert all(p.grad is None for p in net.parameters())
     sync.finish()
     assert len(sync.initial_grads()) == len(sync.params)
+
+
+@pytest.mark.parametrize('how', ['deepcopy', 'pickle', 'save'])
+def test_copies_of_a_network_and_its_flat_gradients(how, tmp_path):
+    """The copy's buffer belongs to the copy's parameters, is filled by the copy's network, and leaves the original alone."""
+    from unet import UNet
+    from unetk.ddp import FlatGrads
+    net = UNet(3, 2, True)
+    sync = FlatGrads(net, grads_to_autograd=False)
+    sync.initial_grads()
+    sync.flat.copy_(torch.arange(sync.total))
+    sync.consume()
+    if how == 'deepcopy':
+        other, twin = copy.deepcopy((net, sync))
+    elif how == 'pickle':
+        other, twin = pickle.loads(pickle.dumps((net, sync)))
+    else:
+        torch.save((net, sync), tmp_path / 'both.pth')               # this test's own file
+        other, twin = torch.load(tmp_path / 'both.pth', weights_only=False)
+    assert {id(p) for p in other.parameters()} == set(twin.offsets) and not set(twin.offsets) & set(sync.offsets)
+    assert [twin.offsets[id(p)] for p in other.parameters()] == [sync.offsets[id(p)] for p in net.parameters()]
+    assert [id(p) for p in other.parameters()] == [id(p) for p in twin.module_order]
+    assert torch.equal(twin.flat, sync.flat) and twin.flat.data_ptr() != sync.flat.data_ptr()
+    for p in twin.params:
+        assert twin.views[p].data_ptr() == twin.flat.data_ptr() + 4 * twin.offsets[id(p)]
+    assert other._initial_grads.__self__ is twin and other._grad_ready_hook.__self__ is twin
+    kept = sync.flat.clone()
+    grads = other._initial_grads()                                   # as the copy's backward pass calls it
+    for layer in FlatGrads._completion_layers(other):
+        for p in layer:
+            grads[p].fill_(2.0)
+        other._grad_ready_hook(layer, grads)
+    twin.finish()
+    twin.bind_param_grads()
+    assert all(bool((p.grad == 2.0).all()) for p in other.parameters()) and all(p.grad is None for p in net.parameters())
+    assert torch.equal(sync.flat, kept)

@@ -164,3 +164,39 @@ def test_discarded_gradients_of_a_flat_buffer_are_not_applied_again(optim, kind)
     fg.initial_grads()
     with pytest.raises(RuntimeError, match='accumulation'):
         fg.initial_grads()
+
+
+@pytest.mark.parametrize('bits', [32, 8])
+def test_copies_of_a_network_and_an_optimizer_on_its_flat_gradients(optim, bits):
+    from unetk.ddp import FlatGrads
+    net, x = make_net(), image()
+    fg = FlatGrads(net, grads_to_autograd=False)
+    opt = optim.AdamW(fg, lr=1e-3, max_norm=1.0, state_bits=bits, seed=4)
+
+    def step(n, o, seed):
+        o.zero_grad()
+        n._initial_grads()                             # as the network's backward pass begins
+        o.fg.flat.copy_(torch.randn(o.fg.total, generator=torch.Generator().manual_seed(seed)))
+        o.step()
+
+    def same(a, b):
+        assert all(torch.equal(p, q) for p, q in zip(a.parameters(), b.parameters()))
+
+    step(net, opt, 0)
+    other, twin = copy.deepcopy((net, opt))
+    assert twin.fg is not fg and other._initial_grads.__self__ is twin.fg
+    opt.step(), twin.step()                            # the gradients at hand, copied too
+    same(net, other)
+    kept, gradients = [p.detach().clone() for p in net.parameters()], fg.flat.clone()
+    for k in (1, 2):                                   # the copy trains alone
+        step(other, twin, k)
+    twin.zero_grad()
+    with torch.autocast('cuda', dtype=torch.bfloat16):
+        other(x).float().square().sum().backward()
+    assert bool(twin.fg.flat.any()) and torch.equal(fg.flat, gradients)
+    assert all(torch.equal(p, q) for p, q in zip(net.parameters(), kept))
+    assert not torch.equal(other.outc.conv.weight, net.outc.conv.weight)
+    for k in (1, 2):
+        step(net, opt, k)
+    same(net, other)
+    assert all(float(o.state[p]['step']) == 4.0 for n, o in ((net, opt), (other, twin)) for p in n.parameters())
