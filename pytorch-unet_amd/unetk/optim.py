@@ -18,6 +18,7 @@ from array import array
 from itertools import chain
 from operator import is_
 
+import numpy as np
 import torch
 
 from . import _native as nat
@@ -291,6 +292,7 @@ class AdamW(torch.optim.Optimizer):
     element's index, for tensors of at least `min_8bit_numel` elements; smaller ones (biases, BatchNorm) keep 32 bits.
     lr: a float, or an fp32 scalar tensor on the device, which a captured graph reads anew at each replay.
 
+    Parameters, moments and step counts that overlap in memory are refused: they would be written in any order.
     The rounding is the same on every rank of a data-parallel job.  A parameter that is laid out anew (net.to(memory_format=...))
     takes its moments along, 8-bit ones rounded to nearest in their new blocks.
     state[p]: `step` (fp32 scalar on the device), `exp_avg`, and `exp_avg_sq` or, in 8 bits, `exp_avg_root` (the square root)
@@ -307,7 +309,7 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f'AdamW: state_bits must be 8 or 32, got {state_bits}')
         self.state_bits, self.min_8bit_numel, self.seed = state_bits, int(min_8bit_numel), int(seed) & 0xFFFFFFFF
         self.total_norm = None
-        self._plan = None
+        self._plan = self._apart = None
         if self.fg is not None:          # net.parameters() order, as a stock optimizer numbers its state
             params = [p for p in self.fg.module_order if id(p) in self.fg.offsets]
             for p in params:             # laid out like its view of the flat gradients
@@ -349,7 +351,7 @@ class AdamW(torch.optim.Optimizer):
 
     def __setstate__(self, state):
         super().__setstate__(state)
-        self._plan = None
+        self._plan = self._apart = None
 
     def zero_grad(self, set_to_none=True):
         if self.fg is not None:
@@ -593,6 +595,7 @@ class _Plan:
             self.tables.append(table)
             self.sets.append((at, dtype_code(dtype), first, len(rs), _address(table)))
             first += len(rs)
+        self._check_apart(opt)
         self.words = [2 * first, 2 * first + sum(int(fn['unetk_grad_partials'](s[3])) for s in self.sets)]
         self.owners = list(opt.state)
         tensors = list(chain.from_iterable(map(dict.values, opt.state.values())))
@@ -606,6 +609,25 @@ class _Plan:
         self.strides = None if self.contiguous else list(map(_get_stride, self.params))
         if opt.fg is not None:
             self.offsets = [4 * opt.fg.offsets[id(p)] for p in self.params]
+
+    def _check_apart(self, opt):
+        """What a step writes must not overlap: the workgroups of a launch come to it in any order."""
+        layout = [(code, table.tobytes()) for (_, code, _, _, _), table in zip(self.sets, self.tables)]
+        if not layout or layout == opt._apart:           # looked at when the tensors last came to lie so
+            return
+        spans = []
+        for (_, code, _, _, _), table in zip(self.sets, self.tables):
+            t = np.frombuffer(table, dtype=np.int64).reshape(-1, 6)
+            codes, numel = t[:, 3] != 0, t[:, 5]
+            size = np.where(codes, 1, 4) * numel
+            blocks = np.where(codes, 2 * -(-numel // BLOCK), 0)
+            for at, nbytes in zip(t[:, :5].T, ((4 if code == nat.F32 else 2) * numel, size, size, blocks, np.full_like(numel, 4))):
+                spans.append(np.stack([at, at + nbytes], 1)[nbytes > 0])
+        spans = np.concatenate(spans)
+        spans = spans[spans[:, 0].argsort()]
+        if (spans[1:, 0] < spans[:-1, 1]).any():
+            raise RuntimeError('AdamW: parameters, moments and step counts must not overlap in memory')
+        opt._apart = layout
 
     def pointers(self, opt):
         """The gradients' pointers if the plan holds for this step, else None."""

@@ -767,6 +767,57 @@ def test_a_limit_of_one_group_alone_is_refused_at_the_step(optim):
     check_step(a + b, before, snapshot(opt, a + b), HYPER, 0.25, 0, opt.total_norm)
 
 
+@pytest.mark.parametrize('bits', [32, 8])
+def test_tensors_that_share_memory_are_refused(optim, bits):
+    """Two workgroups would write the same elements in any order."""
+    def fresh():
+        params = make([5000, 5000, 300], torch.float32)
+        opt = optim.AdamW(params, **HYPER, state_bits=bits)
+        opt.step()
+        return params, opt
+
+    def tied(ps, o):
+        ps[1].data = ps[0].data
+
+    def partly(ps, o):
+        buf = torch.zeros(9999, device='cuda')
+        ps[0].data, ps[1].data = buf[:5000], buf[4999:]
+
+    def one_count(ps, o):
+        o.state[ps[0]]['step'] = o.state[ps[2]]['step']
+
+    def one_moment(ps, o):
+        o.state[ps[0]]['exp_avg'] = o.state[ps[1]]['exp_avg']
+
+    def own_moments(ps, o):
+        o.state[ps[2]]['exp_avg_sq'] = o.state[ps[2]]['exp_avg']
+
+    def parameter_as_moment(ps, o):
+        o.state[ps[2]]['exp_avg'] = ps[2].data
+
+    changes = [tied, partly, one_count, one_moment, own_moments, parameter_as_moment]
+    if bits == 8:
+        def one_scale(ps, o):
+            o.state[ps[0]]['scales'] = o.state[ps[1]]['scales']
+        changes.append(one_scale)
+    for change in changes:
+        params, opt = fresh()
+        change(params, opt)
+        before = snapshot(opt, params)
+        for _ in range(2):
+            with pytest.raises(RuntimeError, match='overlap'):
+                opt.step()
+        for x, y in zip(before, snapshot(opt, params)):
+            assert x['t'] == y['t'] == 1.0 and all(np.array_equal(x[k], y[k]) for k in 'pmv')
+    # side by side is apart
+    params, opt = fresh()
+    buf = torch.randn(10000, device='cuda')
+    params[0].data, params[1].data = buf[:5000], buf[5000:]
+    before = snapshot(opt, params)
+    opt.step()
+    check_step(params, before, snapshot(opt, params), HYPER)
+
+
 # ------------------------------------------------------------------------------------------------------------- clip
 @pytest.mark.parametrize('sizes', list(SIZES))
 @pytest.mark.parametrize('dtype', list(TYPES) + ['mixed'])
