@@ -384,7 +384,8 @@ int unetk_clip_rmsprop_step(float* param, float* grad, float* square_avg, float*
  * grad_scale, found_inf (device, may be NULL): torch.amp.GradScaler's; found_inf != 0 skips the step, its count included.
  *
  * unetk_grad_sumsq + unetk_grad_clip: torch.nn.utils.clip_grad_norm_ (reference train.py:115) by themselves, gradients
- * scaled in place (not written where coef is 1). */
+ * scaled in place (not written where coef is 1).  They must not overlap: unetk_grad_sumsq returns UNETK_ERR_ARG if two do, before
+ * anything is launched.  Nor may what a step writes (parameters, moments, scales, steps), which is the caller's to see to. */
 typedef struct {
   void* param;
   void* exp_avg;    /* fp32, or e4m3 codes */

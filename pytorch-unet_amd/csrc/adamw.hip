@@ -14,6 +14,9 @@
 //   bf16, clip, 17 M elements           8.8           67,    5.7            76      (0.38 GB, 76)
 //   8-bit moments, fp32, U-Net         23             75,    6.6            98      (0.50 GB, 99)
 //   8-bit moments, bf16, wide          41            212,    5.9           254      (1.24 GB, 249)
+#include <algorithm>
+#include <new>
+
 #include "common.h"
 
 namespace {
@@ -505,6 +508,35 @@ int check_grads(void* const* grads, const int64_t* numel, int n, int dtype) {
   return UNETK_OK;
 }
 
+// Gradients that share memory would be scaled in any order, once or twice.  Those of one buffer or one allocation order (rising
+// or falling) need no sorting, which takes 4 us for 130.
+int check_apart(void* const* grads, const int64_t* numel, int n, int dtype) {
+  const uintptr_t es = unetk_esize(dtype);
+  struct Span {
+    uintptr_t begin, end;
+  } last{0, 0};
+  bool rising = true, falling = true, first = true;
+  for (int i = 0; i < n; ++i) {
+    if (numel[i] == 0) continue;
+    const Span s{(uintptr_t)grads[i], (uintptr_t)grads[i] + numel[i] * es};
+    rising &= first || s.begin >= last.end;
+    falling &= first || s.end <= last.begin;
+    last = s;
+    first = false;
+  }
+  if (rising || falling) return UNETK_OK;
+  Span* spans = new (std::nothrow) Span[n];
+  if (!spans) return UNETK_ERR_TOO_LARGE;
+  int k = 0;
+  for (int i = 0; i < n; ++i)
+    if (numel[i]) spans[k++] = Span{(uintptr_t)grads[i], (uintptr_t)grads[i] + numel[i] * es};
+  std::sort(spans, spans + k, [](const Span& a, const Span& b) { return a.begin < b.begin; });
+  bool apart = true;
+  for (int i = 1; i < k; ++i) apart &= spans[i].begin >= spans[i - 1].end;
+  delete[] spans;
+  return apart ? UNETK_OK : UNETK_ERR_ARG;
+}
+
 enum { kStep = 1, kMoments = 2 };                                    // what a call needs of a record
 int check_tensors(const unetk_adamw_tensor* tensors, void* const* grads, int n, int dtype, int need) {
   if (!tensors || !grads || n <= 0) return UNETK_ERR_ARG;
@@ -559,10 +591,11 @@ int64_t unetk_grad_partials(int n_tensors) {
 }
 
 int64_t unetk_grad_sumsq(void* const* grads, const int64_t* numel, int n_tensors, int dtype, double* partials, void* stream) {
-  const int rc = check_grads(grads, numel, n_tensors, dtype);
+  int rc = check_grads(grads, numel, n_tensors, dtype);
   if (rc != UNETK_OK) return rc;
   if (!partials) return UNETK_ERR_ARG;
   if ((uintptr_t)partials & 7) return UNETK_ERR_ALIGN;
+  if ((rc = check_apart(grads, numel, n_tensors, dtype)) != UNETK_OK) return rc;
   int64_t written = 0;
   for (int at = 0; at < n_tensors; at += kGrads) {
     const int n = part_of(n_tensors, at, kGrads);

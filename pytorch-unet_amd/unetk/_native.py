@@ -19,6 +19,8 @@ _ERR = {-1: 'unsupported shape/pitch/channel count', -2: 'unsupported dtype', -3
         -4: 'kernel launch failed', -5: 'bad argument',
         -6: 'problem exceeds the fixed capacity of this no-allocation entry point'}
 
+ERR_ARG = -5
+
 if not os.path.exists(LIB_PATH):
     raise ImportError(f'{LIB_PATH} not found: build it with `make -C pytorch-unet_amd/csrc` '
                       '(or __graft_entry__.build()); there is no non-HIP fallback')

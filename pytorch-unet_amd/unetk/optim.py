@@ -228,8 +228,10 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
         norm = torch.empty((), dtype=torch.float32, device=device)
         at, count = partials.data_ptr(), 0
         for code, n, pointers, numel in sets:
-            count += _written(fn['unetk_grad_sumsq'](_address(pointers), _address(numel), n, code, at + 8 * count, stream),
-                              'unetk_grad_sumsq')
+            written = fn['unetk_grad_sumsq'](_address(pointers), _address(numel), n, code, at + 8 * count, stream)
+            if written == nat.ERR_ARG:                   # all else that it refuses was looked at above
+                raise RuntimeError('clip_grad_norm_: gradients must not overlap in memory')
+            count += _written(written, 'unetk_grad_sumsq')
         if error_if_nonfinite:
             # the very norm that is returned and divided by (fp32: infinite where the sum in fp64 is not), before anything is scaled
             zero = array('q', [0])

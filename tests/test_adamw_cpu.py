@@ -73,6 +73,17 @@ def test_entry_points_refuse_before_launch(nat):
     assert fn['unetk_grad_clip'](a(grad), a(ten), 1, nat.BF16, 64, 3, float('nan'), None, None) == -5
 
 
+@pytest.mark.parametrize('begin,numel', [((64, 64), (10, 10)), ((64, 100), (10, 10)), ((100, 64), (10, 10)), ((64, 200, 72), (10, 3, 1)),
+                                         ((4000, 64, 8000, 3996), (100, 10, 5, 2)), ((64, 4000, 64, 8000), (1, 5, 1000, 7)),
+                                         ((64, 64, 64), (0, 3, 1))])
+def test_gradients_that_overlap_are_refused(nat, begin, numel):
+    b, n = words(*begin), words(*numel)
+    assert nat.fn['unetk_grad_sumsq'](ctypes.addressof(b), ctypes.addressof(n), len(begin), nat.F32, 64, None) == -5
+    if begin == (64, 100):                                                  # in 16 bits 19 elements end at 102
+        n = words(19, 10)
+        assert nat.fn['unetk_grad_sumsq'](ctypes.addressof(b), ctypes.addressof(n), 2, nat.BF16, 64, None) == -5
+
+
 def test_no_cpu_fallback_and_bad_arguments(optim):
     p = torch.nn.Parameter(torch.zeros(4))
     with pytest.raises(RuntimeError, match='cuda'):

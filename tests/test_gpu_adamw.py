@@ -867,6 +867,30 @@ def test_a_norm_beyond_fp32_is_not_finite(optim):
         assert abs(got - want) <= 3 * O.U * want
 
 
+def test_gradients_that_share_memory_are_not_clipped(optim):
+    """They would be scaled once or twice, as the workgroups come; side by side in any order they are apart."""
+    params = [torch.nn.Parameter(torch.zeros(n, device='cuda')) for n in (5000, 5000, 300, 0)]
+    for starts in ((0, 0, 9000, 0), (0, 4999, 12000, 9), (9000, 6000, 8700, 3), (9000, 3000, 8750, 0)):
+        buf = torch.randn(20000, device='cuda')
+        for p, a in zip(params, starts):
+            p.grad = buf[a:a + p.numel()]
+        kept = buf.clone()
+        with pytest.raises(RuntimeError, match='overlap'):
+            optim.clip_grad_norm_(params, 1.0)
+        assert torch.equal(buf, kept)
+    for starts in ((0, 5000, 10000, 7), (5300, 300, 0, 7), (300, 5300, 0, 7), (5000, 0, 10000, 7)):
+        buf = torch.randn(20000, device='cuda')
+        for p, a in zip(params, starts):
+            p.grad = buf[a:a + p.numel()]
+        kept = f64(buf)
+        want = O.norm([kept[:10300]])
+        got = optim.clip_grad_norm_(params, 1.0)
+        assert abs(float(got) - want) <= 3 * O.U * want
+        c = O.clip_coef(want, 1.0)
+        assert (np.abs(f64(buf)[:10300] - kept[:10300] * c) <= np.abs(kept[:10300] * c) * (COEF_ERR + 2 * O.U)).all()
+        assert np.array_equal(f64(buf)[10300:], kept[10300:])
+
+
 def test_more_than_two_to_the_31_elements(optim):
     """Offsets beyond 32 bits: the last elements of a tensor of 2^31 + 4099."""
     n, tail = 2 ** 31 + 4099, 5000
