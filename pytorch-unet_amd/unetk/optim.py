@@ -153,7 +153,7 @@ _TYPES = {torch.float32, torch.bfloat16, torch.float16}
 # one C call per tensor each: a step of small tensors is bound by what the host asks of them
 _get_pointer, _get_numel, _get_device = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device
 _get_contiguous, _get_dtype, _get_stride = torch.Tensor.is_contiguous, torch.Tensor.dtype.__get__, torch.Tensor.stride
-_get_shape = torch.Tensor.shape.__get__
+_get_shape, _get_nbytes = torch.Tensor.shape.__get__, torch.Tensor.nbytes.__get__
 _get_wanted, _get_referent = torch.Tensor.requires_grad.__get__, weakref.ref.__call__
 
 
@@ -606,7 +606,10 @@ class _Plan:
             return
         self.refs = list(map(weakref.ref, tensors))
         self.where = list(map(_get_pointer, self.params)) + list(map(_get_pointer, tensors))
-        self.types, self.numel = list(map(_get_dtype, self.params)), list(map(_get_numel, self.params))
+        # a parameter or gradient that became smaller where it lies must not be stepped with the old table: bytes tell, but not
+        # one 16-bit type from the other
+        self.nbytes, types = list(map(_get_nbytes, self.params)), list(map(_get_dtype, self.params))
+        self.types = types if set(types) - {torch.float32} else None
         self.contiguous = all(map(_get_contiguous, self.params))
         self.strides = None if self.contiguous else list(map(_get_stride, self.params))
         if opt.fg is not None:
@@ -643,7 +646,8 @@ class _Plan:
             return None
         tensors = list(chain.from_iterable(map(dict.values, opt.state.values())))
         if len(tensors) != len(self.refs) or not all(map(is_, tensors, map(_get_referent, self.refs))) or \
-                list(map(_get_pointer, params)) + list(map(_get_pointer, tensors)) != self.where:
+                list(map(_get_pointer, params)) + list(map(_get_pointer, tensors)) != self.where or \
+                list(map(_get_nbytes, params)) != self.nbytes:
             return None
         if not all(map(_get_contiguous, params)) if self.contiguous else list(map(_get_stride, params)) != self.strides:
             return None
@@ -656,7 +660,7 @@ class _Plan:
         if any(p.grad is not None for p in self.absent):
             return None
         try:
-            if list(map(_get_dtype, grads)) != self.types or list(map(_get_numel, grads)) != self.numel:
+            if list(map(_get_nbytes, grads)) != self.nbytes or self.types and list(map(_get_dtype, grads)) != self.types:
                 return None
             if not all(map(_get_contiguous, grads)) if self.contiguous else list(map(_get_stride, grads)) != self.strides:
                 return None

@@ -164,3 +164,38 @@ def test_the_oracles_step_is_torchs():
         assert np.allclose(v['p'], p.detach().numpy(), rtol=1e-12, atol=1e-14)
     st = opt.state[p]
     assert np.allclose(st['exp_avg'], v['m'], rtol=1e-12) and np.allclose(st['exp_avg_sq'], v['v'], rtol=1e-12)
+
+
+@pytest.mark.parametrize('flat', [False, True])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_what_shrinks_where_it_lies_ends_a_plan(optim, flat, dtype):
+    """A parameter or a gradient that is smaller at the same address (pruned and moved back, or of another type): the kernels would
+    write past its end with the table of the step before."""
+    from types import SimpleNamespace
+    params = [torch.nn.Parameter(torch.zeros(n, dtype=dtype)) for n in (40, 30)]
+    opt = SimpleNamespace(fg=None, _apart=None, param_groups=[{'params': params}], state={})
+    for p in params:
+        p.grad = torch.zeros_like(p)
+        opt.state[p] = {'step': torch.zeros(()), 'exp_avg': torch.zeros(p.shape), 'exp_avg_sq': torch.zeros(p.shape)}
+    if flat:
+        opt.fg = SimpleNamespace(offsets={id(params[0]): 0, id(params[1]): 40}, flat=torch.zeros(72, dtype=dtype))
+    plan = optim._Plan(opt, {(0, dtype): [(p, opt.state[p], p.grad) for p in params]}, [])
+    assert plan.pointers(opt) is not None
+    p, whole, half = params[1], params[1].data, torch.bfloat16 if dtype == torch.float32 else torch.float16
+    p.data = whole[:29]
+    assert plan.pointers(opt) is None
+    if dtype == torch.float32:
+        p.data = whole.view(half)[:30]
+        assert plan.pointers(opt) is None
+    p.data = whole
+    assert plan.pointers(opt) is not None
+    if not flat:
+        grad = p.grad.data
+        p.grad.data = grad[:29]
+        assert plan.pointers(opt) is None
+        p.grad.data = grad.view(half)[:30]
+        assert plan.pointers(opt) is None
+        p.grad.data = grad
+        assert plan.pointers(opt) is not None
+        p.grad = None
+        assert plan.pointers(opt) is None

@@ -1052,6 +1052,26 @@ def test_whatever_moves_between_steps_is_noticed(optim, bits):
             o.step()
 
 
+def test_a_parameter_that_was_cut_is_refused_until_all_else_is(optim):
+    params = make([5000, 300], torch.float32)
+    opt = optim.AdamW(params, **HYPER)
+    opt.step()
+    whole = params[0].data
+    params[0].data = whole[:4000]
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match='shape'):
+            opt.step()
+    params[0].grad = params[0].grad[:4000].clone()
+    with pytest.raises(RuntimeError, match='state'):
+        opt.step()
+    for k in ('exp_avg', 'exp_avg_sq'):
+        opt.state[params[0]][k] = opt.state[params[0]][k][:4000]
+    before, kept = snapshot(opt, params), whole[4000:].clone()
+    opt.step()
+    check_step(params, before, snapshot(opt, params), HYPER)
+    assert torch.equal(whole[4000:], kept)
+
+
 def test_frozen_parameters_of_a_flat_buffer_stay(optim):
     from unet import UNet
     from unetk.ddp import FlatGrads
