@@ -380,7 +380,7 @@ int unetk_clip_rmsprop_step(float* param, float* grad, float* square_avg, float*
  *   `partials` is not NULL, sums of squares of the gradients to `partials`.  Returns how many of them it wrote (at most
  *   unetk_grad_partials(n_tensors)) or a negative error.  lr_dev (may be NULL): lr is read from there.
  * unetk_adamw_update: the update; `partials`, `n_partials`: those of ALL sets that the norm covers
- *   (NULL and 0 without a clip).  norm_out (may be NULL) receives the norm.
+ *   (NULL and 0 without a clip).  norm_out (may be NULL) receives the norm.  With 8-bit moments eps is 0 or at least 2^-126.
  * grad_scale, found_inf (device, may be NULL): torch.amp.GradScaler's; found_inf != 0 skips the step, its count included.
  *
  * unetk_grad_sumsq + unetk_grad_clip: torch.nn.utils.clip_grad_norm_ (reference train.py:115) by themselves, gradients

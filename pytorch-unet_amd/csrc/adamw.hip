@@ -15,6 +15,7 @@
 //   8-bit moments, fp32, U-Net         23             75,    6.6            98      (0.50 GB, 99)
 //   8-bit moments, bf16, wide          41            212,    5.9           254      (1.24 GB, 249)
 #include <algorithm>
+#include <cfloat>
 #include <new>
 
 #include "common.h"
@@ -419,7 +420,8 @@ __device__ __forceinline__ void update_block(const Update8Table& tb, int t, long
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     rtop = max(rtop, __float_as_uint(r[k]) & 0x7fffffffu);
-    // one ulp each of the root and the reciprocal; the denominator is no subnormal: a root above zero exceeds 2^-75
+    // one ulp each of the root and the reciprocal; the denominator is no subnormal, which v_rcp_f32 would take for zero: a root
+    // above zero exceeds 2^-75, and eps is zero or normal
     p[k] = fmaf(-c.step_size * m[k], __builtin_amdgcn_rcpf(fmaf(r[k], c.root_correction, b.eps)), elem<T>(pv, k) * c.decay);
     const unsigned h = mix32(place ^ k);
     carry_m[k] = (h << 4 & 0xffff0u) | 8u;
@@ -671,6 +673,7 @@ int unetk_adamw_update(const unetk_adamw_tensor* tensors, void* const* grads, in
   if (rc == UNETK_OK) rc = check_clip(partials, n_partials, max_norm);
   if (rc != UNETK_OK) return rc;
   if (!coefs) return UNETK_ERR_ARG;
+  if (eps > 0.0 && eps < FLT_MIN && any_scales(tensors, n_tensors)) return UNETK_ERR_ARG;        // see update_block
   const Betas b{(float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps};
   const Clip clip{partials, (int)n_partials, (float)max_norm, grad_scale, norm_out};
   for (int at = (n_tensors - 1) / kUpdate * kUpdate; at >= 0; at -= kUpdate) {

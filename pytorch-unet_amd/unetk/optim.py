@@ -338,13 +338,13 @@ class AdamW(torch.optim.Optimizer):
             if p.device != next(q for h in self.param_groups for q in h['params']).device:
                 raise RuntimeError('AdamW: parameters must be on one device')
 
-    @staticmethod
-    def _check_hyperparameters(g, groups):
+    def _check_hyperparameters(self, g, groups):
         for k in ('lr', 'eps', 'weight_decay'):
             if not isinstance(g[k], torch.Tensor) and not g[k] >= 0:
                 raise ValueError(f'AdamW: {k} must not be negative, got {g[k]}')
         if not all(0.0 <= b < 1.0 for b in g['betas']):
             raise ValueError(f"AdamW: betas must lie in [0, 1), got {g['betas']}")
+        _usable_eps(g, self.state_bits)
         _common_max_norm(groups)
 
     def __getstate__(self):
@@ -503,7 +503,7 @@ class AdamW(torch.optim.Optimizer):
     def _launch(self, plan, pointers):
         stream, device = stream_ptr(), plan.device
         # all that can be wrong with the groups is found here: once a launch has counted, the step has to go through
-        hyper = [_hyperparameters(self.param_groups[at], device) for at, _, _, _, _ in plan.sets]
+        hyper = [_hyperparameters(self.param_groups[at], device, self.state_bits) for at, _, _, _, _ in plan.sets]
         max_norm = _common_max_norm(self.param_groups)
         grad_scale, found_inf = getattr(self, 'grad_scale', None), getattr(self, 'found_inf', None)
         for t in (grad_scale, found_inf):
@@ -542,7 +542,15 @@ def _common_max_norm(groups):
     return max_norm
 
 
-def _hyperparameters(group, device):
+def _usable_eps(group, bits):
+    """The 8-bit update takes a reciprocal whose argument must not be subnormal."""
+    eps = float(group['eps'])
+    if bits == 8 and 0.0 < eps < 2.0 ** -126:
+        raise ValueError(f'AdamW: with 8-bit moments eps must be 0 or at least 2^-126, got {eps}')
+    return eps
+
+
+def _hyperparameters(group, device, bits):
     """(lr, pointer to an lr on the device or None, beta1, beta2, eps, weight_decay) as a launch takes them."""
     lr, lr_ptr = group['lr'], None
     if isinstance(lr, torch.Tensor) and lr.is_cuda:
@@ -550,7 +558,7 @@ def _hyperparameters(group, device):
             raise RuntimeError("AdamW: a tensor lr must be an fp32 scalar on the parameters' device")
         lr, lr_ptr = 0.0, lr.data_ptr()
     beta1, beta2 = group['betas']
-    return float(lr), lr_ptr, float(beta1), float(beta2), float(group['eps']), float(group['weight_decay'])
+    return float(lr), lr_ptr, float(beta1), float(beta2), _usable_eps(group, bits), float(group['weight_decay'])
 
 
 def _all_usual(rows):

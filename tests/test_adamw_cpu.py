@@ -84,6 +84,17 @@ def test_gradients_that_overlap_are_refused(nat, begin, numel):
         assert nat.fn['unetk_grad_sumsq'](ctypes.addressof(b), ctypes.addressof(n), 2, nat.BF16, 64, None) == -5
 
 
+def test_a_subnormal_eps_with_8bit_moments_is_refused(nat, optim):
+    """The reciprocal of a subnormal is infinite in the 8-bit update: 0 / eps would be NaN where a gradient was never seen."""
+    row, grad, a = words(*ROW), words(64), ctypes.addressof
+    for eps in (1e-40, 1e-46, 2.0 ** -126 * (1 - 2.0 ** -24)):
+        assert nat.fn['unetk_adamw_update'](a(row), a(grad), 1, nat.F32, 0.9, 0.999, eps, None, None, 64, None, 0, 1.0, None, None) == -5
+        with pytest.raises(ValueError, match='eps'):
+            optim._usable_eps({'eps': eps}, 8)
+        assert optim._usable_eps({'eps': eps}, 32) == eps
+    assert optim._usable_eps({'eps': 0}, 8) == 0.0 and optim._usable_eps({'eps': 2.0 ** -126}, 8) == 2.0 ** -126
+
+
 def test_no_cpu_fallback_and_bad_arguments(optim):
     p = torch.nn.Parameter(torch.zeros(4))
     with pytest.raises(RuntimeError, match='cuda'):

@@ -818,6 +818,30 @@ def test_tensors_that_share_memory_are_refused(optim, bits):
     check_step(params, before, snapshot(opt, params), HYPER)
 
 
+@pytest.mark.parametrize('bits', [32, 8])
+def test_the_smallest_eps(optim, bits):
+    """Elements whose gradient is always zero stay (but for the decay) whatever eps is above zero; below fp32's normal numbers it is
+    refused with 8 bits, before anything has counted."""
+    for eps in (2.0 ** -126, 1e-30) + ((1e-40,) if bits == 32 else ()):
+        hyper = dict(HYPER, eps=eps)
+        params = make([5000], torch.float32)
+        params[0].grad[::3] = 0.0
+        opt = optim.AdamW(params, **hyper, state_bits=bits, min_8bit_numel=1)
+        for _ in range(2):
+            before = snapshot(opt, params)
+            opt.step()
+            check_step(params, before, snapshot(opt, params), hyper)
+    if bits == 8:
+        with pytest.raises(ValueError, match='eps'):
+            optim.AdamW(params, eps=1e-40, state_bits=8)
+        opt.param_groups[0]['eps'] = 1e-40
+        with pytest.raises(ValueError, match='eps'):
+            opt.step()
+        assert float(opt.state[params[0]]['step']) == 2.0
+        opt.param_groups[0]['eps'] = 1e-8
+        opt.step()
+
+
 # ------------------------------------------------------------------------------------------------------------- clip
 @pytest.mark.parametrize('sizes', list(SIZES))
 @pytest.mark.parametrize('dtype', list(TYPES) + ['mixed'])
