@@ -56,12 +56,13 @@ def planned(packed):
         _PLANNED = prev
 
 
-def wrote_in_place(params):
+def wrote_in_place(params, stream):
     """Kernels wrote `params` behind PyTorch's back: bump their version counters like any in-place op would, so autograd's
     checks and packed_weight() see it.  A graph that is captured here writes them again at every replay and bumps nothing then:
-    such parameters are marked, and no version is trusted to tell whether a packing of them is current."""
+    such parameters are marked, and no version is trusted to tell whether a packing of them is current.  stream: the handle of the
+    current stream (0, the default one, is never captured, and asking costs 2 us of a small step's 30)."""
     torch.autograd.graph.increment_version(params)
-    if torch.cuda.is_current_stream_capturing():
+    if stream and torch.cuda.is_current_stream_capturing():
         for p in params:
             p._unetk_graph_writes = True
 

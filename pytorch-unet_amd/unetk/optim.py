@@ -139,7 +139,7 @@ class ClipRMSprop(torch.optim.Optimizer):
                                             float(g['lr']), float(g['alpha']), float(g['eps']),
                                             float(g['weight_decay']), float(g['momentum']), stream_ptr()),
               'unetk_clip_rmsprop_step')
-        wrote_in_place(self.fg.params)
+        wrote_in_place(self.fg.params, stream_ptr())
         self._steps += 1
         self.fg.consume()
         return None
@@ -154,7 +154,7 @@ _TYPES = {torch.float32, torch.bfloat16, torch.float16}
 _get_pointer, _get_numel, _get_device = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device
 _get_contiguous, _get_dtype, _get_stride = torch.Tensor.is_contiguous, torch.Tensor.dtype.__get__, torch.Tensor.stride
 _get_shape, _get_nbytes = torch.Tensor.shape.__get__, torch.Tensor.nbytes.__get__
-_get_wanted, _get_referent = torch.Tensor.requires_grad.__get__, weakref.ref.__call__
+_get_wanted = torch.Tensor.requires_grad.__get__
 
 
 def _address(words):
@@ -457,8 +457,9 @@ class AdamW(torch.optim.Optimizer):
                 with torch.no_grad():
                     plan, pointers, copies = self._make_plan()
             if plan.params:
-                self._launch(plan, pointers)
-                wrote_in_place(plan.params)
+                stream = stream_ptr()
+                self._launch(plan, pointers, stream)
+                wrote_in_place(plan.params, stream)
             else:                                        # no gradients: a norm of zero, not an earlier step's
                 limit = _common_max_norm(self.param_groups)
                 self.total_norm = None if limit is None else torch.zeros((), dtype=torch.float32, device=device)
@@ -500,8 +501,8 @@ class AdamW(torch.optim.Optimizer):
             sets.setdefault((at, p.dtype), []).append((p, st, g))
         return _Plan(self, sets, absent), array('q', [g.data_ptr() for rs in sets.values() for _, _, g in rs]), copies
 
-    def _launch(self, plan, pointers):
-        stream, device = stream_ptr(), plan.device
+    def _launch(self, plan, pointers, stream):
+        device = plan.device
         # all that can be wrong with the groups is found here: once a launch has counted, the step has to go through
         hyper = [_hyperparameters(self.param_groups[at], device, self.state_bits) for at, _, _, _, _ in plan.sets]
         max_norm = _common_max_norm(self.param_groups)
@@ -537,7 +538,7 @@ def _common_max_norm(groups):
         max_norm = float(max_norm)
         if not max_norm > 0:
             raise ValueError(f'AdamW: max_norm must be positive or None, got {max_norm}')
-    if any(g['max_norm'] != max_norm for g in groups):
+    if len(groups) > 1 and any(g['max_norm'] != max_norm for g in groups):
         raise ValueError('AdamW: the clip is over all groups: max_norm must be the same in each')
     return max_norm
 
@@ -612,7 +613,8 @@ class _Plan:
         self.usable = all(map(torch.is_tensor, tensors))      # a user may keep other things there: then every step looks anew
         if not self.usable:
             return
-        self.refs = list(map(weakref.ref, tensors))
+        self.ids, self.gone = list(map(id, tensors)), []
+        self.refs = [weakref.ref(t, self.gone.append) for t in tensors]          # an id is its tensor's while that lives
         self.where = list(map(_get_pointer, self.params)) + list(map(_get_pointer, tensors))
         # a parameter or gradient that became smaller where it lies must not be stepped with the old table: bytes tell, but not
         # one 16-bit type from the other
@@ -653,7 +655,7 @@ class _Plan:
         if len(opt.state) != len(self.owners) or not all(map(is_, opt.state, self.owners)):
             return None
         tensors = list(chain.from_iterable(map(dict.values, opt.state.values())))
-        if len(tensors) != len(self.refs) or not all(map(is_, tensors, map(_get_referent, self.refs))) or \
+        if self.gone or list(map(id, tensors)) != self.ids or \
                 list(map(_get_pointer, params)) + list(map(_get_pointer, tensors)) != self.where or \
                 list(map(_get_nbytes, params)) != self.nbytes:
             return None
