@@ -385,7 +385,9 @@ int unetk_clip_rmsprop_step(float* param, float* grad, float* square_avg, float*
  *
  * unetk_grad_sumsq + unetk_grad_clip: torch.nn.utils.clip_grad_norm_ (reference train.py:115) by themselves, gradients
  * scaled in place (not written where coef is 1).  They must not overlap: unetk_grad_sumsq returns UNETK_ERR_ARG if two do, before
- * anything is launched.  Nor may what a step writes (parameters, moments, scales, steps), which is the caller's to see to. */
+ * anything is launched.  Nor may what a step writes (parameters, moments, scales, steps), which is for the caller to see to:
+ * unetk_adamw_overlaps (host only) returns 1 if two of the records' arrays share memory, 0 if not; element_size: bytes of each
+ * record's parameter. */
 typedef struct {
   void* param;
   void* exp_avg;    /* fp32, or e4m3 codes */
@@ -395,6 +397,7 @@ typedef struct {
   int64_t numel;
 } unetk_adamw_tensor;
 int64_t unetk_grad_partials(int n_tensors);
+int64_t unetk_adamw_overlaps(const unetk_adamw_tensor* tensors, const uint8_t* element_size, int n_tensors);
 int64_t unetk_grad_sumsq(void* const* grads, const int64_t* numel, int n_tensors, int dtype, double* partials, void* stream);
 int unetk_grad_clip(void* const* grads, const int64_t* numel, int n_tensors, int dtype, const double* partials,
                     int64_t n_partials, double max_norm, float* norm_out, void* stream);

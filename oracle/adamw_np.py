@@ -46,6 +46,7 @@ def step(p, g, m, v, t, lr, b1, b2, eps, wd, factor=1.0, factor_err=0.0, half=0.
 
 # ---- 8-bit codes
 def mix(h):
+    """The 32-bit MurmurHash3's finalizer."""
     h = np.asarray(h, dtype=np.uint64) & 0xFFFFFFFF
     h = ((h ^ (h >> np.uint64(16))) * np.uint64(0x85EBCA6B)) & np.uint64(0xFFFFFFFF)
     h = ((h ^ (h >> np.uint64(13))) * np.uint64(0xC2B2AE35)) & np.uint64(0xFFFFFFFF)

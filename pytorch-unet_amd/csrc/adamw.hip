@@ -8,12 +8,13 @@
 // Everything here is bound by HBM (a copy of 2 GB reaches 5.0 TB/s on this card, a sum 4.0 to 6.3).  Measured, three sets of
 // inputs in turn so that no step finds its own in the 256 MiB last-level cache; "U-Net": 31 M elements in 64 tensors, "wide":
 // 124 M; bytes are what a step has to read and write once, the second read of the gradients not counted:
-//                                   sums + counts    update                whole step
-//   fp32, clip, U-Net                  21.5 us       139 us, 6.2 TB/s      161 us   (0.87 GB, 174 us at the copy's rate)
-//   fp32, clip, wide                   80            594,    5.9           675      (3.48 GB, 695)
-//   bf16, clip, 17 M elements           8.8           67,    5.7            76      (0.38 GB, 76)
+//                                   sums + counts    update                both
+//   fp32, clip, U-Net                  22 us         139 us, 6.3 TB/s      161 us   (0.87 GB, 174 us at the copy's rate)
+//   fp32, clip, wide                   80            596,    5.8           676      (3.48 GB, 695)
+//   bf16, clip, 17 M elements           9             65,    5.8            74      (0.38 GB, 76)
 //   8-bit moments, fp32, U-Net         23             75,    6.6            98      (0.50 GB, 99)
-//   8-bit moments, bf16, wide          41            212,    5.9           254      (1.24 GB, 249)
+//   8-bit moments, bf16, wide          43            214,    5.8           257      (1.24 GB, 249)
+// (profiles/adamw_kernels.txt; what other grids, chunks and cache policies take: profiles/adamw_sweeps.txt)
 #include <algorithm>
 #include <cfloat>
 #include <new>
@@ -26,12 +27,14 @@ constexpr int kGrads = 192;       // tensors a launch that needs their gradients
 constexpr int kPrepare = 128;     // 28 bytes each
 constexpr int kSteps = 256;       // a prepare without sums: 8 bytes and a thread each
 constexpr int kUpdate = 64;       // 52 bytes each
-constexpr int kChunk = 4096;      // elements, 16 per thread; 2048 / 8192: wide 738 / 723 us (724), 190 tensors 52 / 61 us (54)
+constexpr int kChunk = 4096;      // elements, 16 per thread; 2048 / 8192: wide 672 / 693 us (678), wide bf16 in 8 bits 277 / 264
+                                  // (262 to 270), 190 tensors 48 / 56 (48), clip of 130 bf16 tensors 37 / 35 (35)
 constexpr int kBlock = 256;       // elements that share a scale: one wave, four per lane
-// Workgroups at most.  The sums: 512 / 1024 / 2048 read 118 MiB in 23.8 / 21.8 / 22.4 us, and every later workgroup adds up that
-// many partials.  The clip does not mind (512 to 4096: +-1 %).  The update wants few streams at once, 512 / 768 / 1024 / 2048
-// take 166 / 163 / 165 / 169 us for the U-Net and 662 / 676 / 685 / 724 for its wide form, 83 / 76 / 77 / 81 in bf16.  The 8-bit
-// one has arithmetic to hide and evens out its end with many: 2048 / 4096 / 8192 take 102.5 / 98.5 / 97.9 and 293 / 292 / 274 us.
+// Workgroups at most.  The sums: every later workgroup adds up as many partials; with 512 / 1024 / 2048 a step takes 165 / 162 /
+// 164 us for the U-Net and 684 / 678 / 694 for its wide form.  The clip does not mind (512 to 4096: 1 % for the U-Net).  The
+// update wants few streams at once, 512 / 768 / 1024 / 2048 take 164 / 162 / 163 / 170 us for the U-Net, 671 / 678 / 686 / 725
+// for its wide form, 80 / 75 / 76 / 78 in bf16.  The 8-bit one has arithmetic to hide and evens out its end with many: 2048 /
+// 4096 / 8192 take 102 / 99 / 99 and 275 / 267 / 262 to 270 us.
 constexpr int kSumsqGrid = 1024;
 constexpr int kClipGrid = 2048;
 constexpr int kUpdateGrid = 768;
@@ -105,8 +108,8 @@ template <typename T> struct Raw4 { typedef u16x4u type; };
 template <> struct Raw4<float> { typedef f32x4u type; };
 
 // FULL: all four exist; otherwise those before n, zeros behind.  ONCE: nothing of this step reads them again, so they pass by
-// the caches, as all stores do, and leave the gradients there between the sums and the update: the U-Net's step falls from 195
-// to 172 us, the wide one's from 792 to 727; with the gradients passing by as well it is 181 and 714 instead of 161 and 675.
+// the caches, as all stores do, and leave the gradients there between the sums and the update: the U-Net's step falls from 186
+// to 162 us, the wide one's from 766 to 678; with the sums' reads passing by as well it is 181 and 714 to 721.
 template <typename T, bool FULL, bool ONCE = false>
 __device__ __forceinline__ typename Raw4<T>::type load4(const void* base, long i, long n) {
   typedef typename Raw4<T>::type V;
@@ -169,8 +172,9 @@ template <typename T, bool FULL> __device__ __forceinline__ double chunk_sumsq(c
     }
   return s;
 }
-// One read of the gradients at 5.7 (124 MB) to 6.3 TB/s (1.6 GB); a workgroup's sum goes to a slot of its own, so that the norm
-// does not depend on who comes first.
+// One read of the gradients: 124 MB that a kernel before wrote in 21 to 22 us (5.7 TB/s), by themselves or in a step; 31 us right
+// behind the clip of other gradients, whose stores are still on their way to memory.  A workgroup's sum goes to a slot of its own,
+// so that the norm does not depend on who comes first.
 template <typename T, typename Table> __device__ __forceinline__ void write_partial(const Table& tb, double* partials) {
   const Owners owners(tb.c);
   double s = 0.0;
@@ -188,6 +192,8 @@ template <typename T> __global__ __launch_bounds__(256) void grad_sumsq_kernel(G
   write_partial<T>(tb, partials);
 }
 
+// The finalizer of the 32-bit MurmurHash3: a published mixing in which every input bit flips every output bit about half of the
+// time.
 __device__ __forceinline__ unsigned mix32(unsigned h) {
   h = (h ^ (h >> 16)) * 0x85EBCA6Bu;
   h = (h ^ (h >> 13)) * 0xC2B2AE35u;
@@ -224,8 +230,11 @@ __global__ __launch_bounds__(256) void adamw_prepare_kernel(PrepareTable tb, int
 }
 
 // What the gradient is multiplied by.  Every workgroup sums the partials in the same order, so all agree to the bit, and no
-// launch in between has to (a kernel of one workgroup costs 3 us, these sums under 1).  A norm that is
-// not a number makes the coefficient one that is not either, as clip_grad_norm_ does.
+// launch in between has to (a kernel of one workgroup costs 3 us; for up to 128 tensors these sums do not show beside the read
+// of the gradients).  Their cost grows with the number of partials times that of the launches: over 1000 / 2000 tensors of 0.5 M
+// elements a step takes 9 / 130 us more than one without a clip and a read of the gradients at 6 TB/s (2.9 / 5.9 ms in all), with
+// 8-bit moments and their larger grid 230 / 1260 us more (2.0 / 4.8 ms).  A norm that is not a number makes the coefficient one
+// that is not either, as clip_grad_norm_ does.
 __device__ __forceinline__ float grad_factor(const Clip& c) {
   const double inv_scale = c.grad_scale ? 1.0 / (double)*c.grad_scale : 1.0;
   if (!c.partials) return (float)inv_scale;
@@ -239,8 +248,8 @@ __device__ __forceinline__ float grad_factor(const Clip& c) {
   return (float)(coef * inv_scale);
 }
 
-// Second pass of the clip: 39 us for 124 MB of gradients (6.3 TB/s read and written, the read mostly from the last-level cache),
-// from the last chunk the sums read to the first, as in the updates.
+// Second pass of the clip: 38 to 39 us for 124 MB of gradients (6.4 TB/s read and written, the read mostly from the last-level
+// cache), from the last chunk the sums read to the first, as in the updates.
 template <typename T, bool FULL> __device__ __forceinline__ void clip_chunk(void* grad, long base, long n, float coef) {
   typename Raw4<T>::type g[kChunk / 1024];
 #pragma unroll
@@ -299,7 +308,7 @@ __device__ __forceinline__ void update_chunk(const UpdateTable& tb, int t, long 
   }
 }
 
-// From the last chunk to the first: what the sums read last is still in the last-level cache (forwards: up to 3 % more).
+// From the last chunk to the first: what the sums read last is still in the last-level cache (forwards: up to 6 % more).
 template <typename T>
 __global__ __launch_bounds__(256) void adamw_update_kernel(UpdateTable tb, Betas b, const Coefs* __restrict__ coefs,
                                                            const float* __restrict__ found_inf, Clip clip) {
@@ -510,17 +519,27 @@ int check_grads(void* const* grads, const int64_t* numel, int n, int dtype) {
   return UNETK_OK;
 }
 
+struct Span {
+  uintptr_t begin, end;
+};
+// Whether two of the spans share a byte; sorts them.
+bool any_overlap(Span* spans, int n) {
+  std::sort(spans, spans + n, [](const Span& a, const Span& b) { return a.begin < b.begin; });
+  for (int i = 1; i < n; ++i)
+    if (spans[i].begin < spans[i - 1].end) return true;
+  return false;
+}
+
 // Gradients that share memory would be scaled in any order, once or twice.  Those of one buffer or one allocation order (rising
-// or falling) need no sorting, which takes 4 us for 130.
+// or falling) need no sorting, which takes 6 us for 130 in random order.
 int check_apart(void* const* grads, const int64_t* numel, int n, int dtype) {
   const uintptr_t es = unetk_esize(dtype);
-  struct Span {
-    uintptr_t begin, end;
-  } last{0, 0};
+  const auto span = [&](int i) { return Span{(uintptr_t)grads[i], (uintptr_t)grads[i] + numel[i] * es}; };
+  Span last{0, 0};
   bool rising = true, falling = true, first = true;
   for (int i = 0; i < n; ++i) {
     if (numel[i] == 0) continue;
-    const Span s{(uintptr_t)grads[i], (uintptr_t)grads[i] + numel[i] * es};
+    const Span s = span(i);
     rising &= first || s.begin >= last.end;
     falling &= first || s.end <= last.begin;
     last = s;
@@ -531,12 +550,10 @@ int check_apart(void* const* grads, const int64_t* numel, int n, int dtype) {
   if (!spans) return UNETK_ERR_TOO_LARGE;
   int k = 0;
   for (int i = 0; i < n; ++i)
-    if (numel[i]) spans[k++] = Span{(uintptr_t)grads[i], (uintptr_t)grads[i] + numel[i] * es};
-  std::sort(spans, spans + k, [](const Span& a, const Span& b) { return a.begin < b.begin; });
-  bool apart = true;
-  for (int i = 1; i < k; ++i) apart &= spans[i].begin >= spans[i - 1].end;
+    if (numel[i]) spans[k++] = span(i);
+  const bool overlap = any_overlap(spans, k);
   delete[] spans;
-  return apart ? UNETK_OK : UNETK_ERR_ARG;
+  return overlap ? UNETK_ERR_ARG : UNETK_OK;
 }
 
 enum { kStep = 1, kMoments = 2 };                                    // what a call needs of a record
@@ -630,6 +647,27 @@ int unetk_grad_clip(void* const* grads, const int64_t* numel, int n_tensors, int
     UNETK_CHECK_LAUNCH();
   }
   return UNETK_OK;
+}
+
+int64_t unetk_adamw_overlaps(const unetk_adamw_tensor* tensors, const uint8_t* element_size, int n_tensors) {
+  if (!tensors || !element_size || n_tensors <= 0 || n_tensors > INT32_MAX / 5) return UNETK_ERR_ARG;
+  Span* spans = new (std::nothrow) Span[5 * n_tensors];
+  if (!spans) return UNETK_ERR_TOO_LARGE;
+  int k = 0;
+  const auto add = [&](const void* p, int64_t bytes) {
+    if (bytes > 0) spans[k++] = Span{(uintptr_t)p, (uintptr_t)p + bytes};
+  };
+  for (int i = 0; i < n_tensors; ++i) {
+    const unetk_adamw_tensor& t = tensors[i];
+    add(t.step, sizeof(float));
+    add(t.param, t.numel * element_size[i]);
+    add(t.exp_avg, t.numel * (t.scales ? 1 : 4));
+    add(t.exp_avg_sq, t.numel * (t.scales ? 1 : 4));
+    if (t.scales) add(t.scales, (t.numel + kBlock - 1) / kBlock * 2);
+  }
+  const bool overlap = any_overlap(spans, k);
+  delete[] spans;
+  return overlap;
 }
 
 int64_t unetk_adamw_prepare(const unetk_adamw_tensor* tensors, void* const* grads, int n_tensors, int dtype, double lr,

@@ -18,7 +18,6 @@ from array import array
 from itertools import chain
 from operator import is_
 
-import numpy as np
 import torch
 
 from . import _native as nat
@@ -630,17 +629,11 @@ class _Plan:
         layout = [(code, table.tobytes()) for (_, code, _, _, _), table in zip(self.sets, self.tables)]
         if not layout or layout == opt._apart:           # looked at when the tensors last came to lie so
             return
-        spans = []
-        for (_, code, _, _, _), table in zip(self.sets, self.tables):
-            t = np.frombuffer(table, dtype=np.int64).reshape(-1, 6)
-            codes, numel = t[:, 3] != 0, t[:, 5]
-            size = np.where(codes, 1, 4) * numel
-            blocks = np.where(codes, 2 * -(-numel // BLOCK), 0)
-            for at, nbytes in zip(t[:, :5].T, ((4 if code == nat.F32 else 2) * numel, size, size, blocks, np.full_like(numel, 4))):
-                spans.append(np.stack([at, at + nbytes], 1)[nbytes > 0])
-        spans = np.concatenate(spans)
-        spans = spans[spans[:, 0].argsort()]
-        if (spans[1:, 0] < spans[:-1, 1]).any():
+        rows, size = array('q'), array('B')
+        for (_, code, _, n, _), table in zip(self.sets, self.tables):
+            rows.extend(table)
+            size.extend([4 if code == nat.F32 else 2] * n)
+        if _written(fn['unetk_adamw_overlaps'](_address(rows), _address(size), len(size)), 'unetk_adamw_overlaps'):
             raise RuntimeError('AdamW: parameters, moments and step counts must not overlap in memory')
         opt._apart = layout
 

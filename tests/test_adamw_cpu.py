@@ -84,6 +84,40 @@ def test_gradients_that_overlap_are_refused(nat, begin, numel):
         assert nat.fn['unetk_grad_sumsq'](ctypes.addressof(b), ctypes.addressof(n), 2, nat.BF16, 64, None) == -5
 
 
+def test_overlaps_of_what_a_step_writes(nat):
+    """Every pair of arrays of two records, one byte too far and one byte apart, in both forms and element sizes."""
+    def overlaps(records, sizes):
+        flat = words(*[w for r in records for w in r])
+        es = (ctypes.c_uint8 * len(sizes))(*sizes)
+        return nat.fn['unetk_adamw_overlaps'](ctypes.addressof(flat), ctypes.addressof(es), len(sizes))
+
+    n = 300
+    for es in (4, 2):
+        for codes in (False, True):
+            span = [n * es, n * (1 if codes else 4), n * (1 if codes else 4), 4 if codes else 0, 4]       # two blocks of scales
+            def record(at):
+                return [at, at + 10000, at + 20000, at + 30000 if codes else 0, at + 40000, n]
+            a, b = record(1 << 20), record(1 << 24)
+            assert overlaps([a, b], [es, es]) == 0 and overlaps([a], [es]) == 0
+            for i in range(5):
+                for j in range(5):
+                    if span[i] == 0 or span[j] == 0:
+                        continue
+                    b2 = list(b)
+                    b2[j] = a[i] + span[i]
+                    assert overlaps([a, b2], [es, es]) == 0 and overlaps([b2, a], [es, es]) == 0
+                    b2[j] -= 1
+                    assert overlaps([a, b2], [es, es]) == 1 and overlaps([b2, a], [es, es]) == 1
+                    if i < j:
+                        a2 = list(a)
+                        a2[j] = a[i]
+                        assert overlaps([a2], [es]) == 1
+            empty = [*b[:5], 0]
+            assert overlaps([a, [a[0], a[1], a[2], a[3], b[4], 0]], [es, es]) == 0                       # no elements: only the count
+            assert overlaps([a, [*empty[:4], a[4], 0]], [es, es]) == 1
+    assert overlaps([a], []) == -5 and nat.fn['unetk_adamw_overlaps'](None, 64, 1) == -5 and nat.fn['unetk_adamw_overlaps'](64, None, 1) == -5
+
+
 def test_a_subnormal_eps_with_8bit_moments_is_refused(nat, optim):
     """The reciprocal of a subnormal is infinite in the 8-bit update: 0 / eps would be NaN where a gradient was never seen."""
     row, grad, a = words(*ROW), words(64), ctypes.addressof
