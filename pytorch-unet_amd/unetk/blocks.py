@@ -12,6 +12,7 @@ Reference semantics restated (file:line into the reference):
 """
 import contextlib
 import os
+import threading
 
 import torch
 
@@ -40,20 +41,23 @@ def activation_dtype(x):
     raise RuntimeError(f'unsupported activation dtype {x.dtype}')
 
 
-# (module, kind, dtype) of the packed weights that pack_all has brought up to date for the whole-network pass that runs now
-_PLANNED = frozenset()
+class _Pass(threading.local):
+    """The whole-network pass that this thread runs (backward passes run on autograd's own threads)."""
+    packed = frozenset()        # (module, kind, dtype) of the packed weights that pack_all has brought up to date for it
+
+
+_PASS = _Pass()
 _RECORDED = -1                  # in the place of a version: this packing was recorded into a graph, not done
 
 
 @contextlib.contextmanager
 def planned(packed):
     """While a whole-network pass runs: packed_weight() takes what pack_all (which returned `packed`) prepared for it."""
-    global _PLANNED
-    prev, _PLANNED = _PLANNED, packed
+    prev, _PASS.packed = _PASS.packed, packed
     try:
         yield
     finally:
-        _PLANNED = prev
+        _PASS.packed = prev
 
 
 def wrote_in_place(params, stream):
@@ -80,7 +84,7 @@ def packed_weight(mod, kind, dtype, c_out, c_in):
     cache = mod.__dict__.setdefault('_unetk_pack', {})
     key = (kind, dtype)
     hit = cache.get(key)
-    if (mod, kind, dtype) in _PLANNED and hit is not None and hit[0] in (w._version, _RECORDED) and hit[1] == w.data_ptr():
+    if (mod, kind, dtype) in _PASS.packed and hit is not None and hit[0] in (w._version, _RECORDED) and hit[1] == w.data_ptr():
         return hit[2]
     if torch.cuda.is_current_stream_capturing():
         return ops.pack_weight(kind, w, c_out, c_in, dtype)      # the graph's own: nothing eager may take it for done

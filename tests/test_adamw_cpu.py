@@ -244,3 +244,30 @@ def test_what_shrinks_where_it_lies_ends_a_plan(optim, flat, dtype):
         assert plan.pointers(opt) is not None
         p.grad = None
         assert plan.pointers(opt) is None
+
+
+def test_a_pass_over_the_network_is_its_threads_own(nat):
+    """Two passes that overlap in time, and end in the order they began, leave nothing behind."""
+    import threading
+    from unetk import blocks
+    inside, leave, seen = threading.Event(), threading.Event(), []
+
+    def other():
+        with blocks.planned(frozenset({'b'})):
+            inside.set()
+            leave.wait(10)
+            seen.append(blocks._PASS.packed)
+        seen.append(blocks._PASS.packed)
+
+    t = threading.Thread(target=other)
+    with blocks.planned(frozenset({'a'})):
+        t.start()
+        inside.wait(10)
+        assert blocks._PASS.packed == {'a'}
+        with pytest.raises(ZeroDivisionError):
+            with blocks.planned(frozenset({'c'})):
+                1 / 0
+        assert blocks._PASS.packed == {'a'}
+    leave.set()
+    t.join()
+    assert seen == [{'b'}, frozenset()] and blocks._PASS.packed == frozenset()
