@@ -291,6 +291,7 @@ class AdamW(torch.optim.Optimizer):
     state_bits: 32 keeps `exp_avg` and `exp_avg_sq` in fp32 whatever the parameter's type.  8 keeps them as fp8 codes with a
     power-of-two scale per 256 elements (2.02 instead of 8 bytes a parameter), rounded stochastically from `seed`, the step and the
     element's index, for tensors of at least `min_8bit_numel` elements; smaller ones (biases, BatchNorm) keep 32 bits.
+    eps is then 0 or at least 2^-126.
     lr: a float, or an fp32 scalar tensor on the device, which a captured graph reads anew at each replay.
 
     Parameters, moments and step counts that overlap in memory are refused: they would be written in any order.
